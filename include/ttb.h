@@ -28,7 +28,7 @@ typedef enum {
   TTB_ERR_UNSUPPORTED = 3,  /* dtype / shape combination has no kernel                                 */
   TTB_ERR_OOM = 4,          /* the device pool could not satisfy an allocation                         */
   TTB_ERR_DEVICE_WAIT = 5,  /* a bounded device-side wait (mbarrier) expired; results are undefined    */
-  TTB_ERR_BAD_INDEX = 6     /* an embedding id was outside its table (it was clamped, not trapped on)  */
+  TTB_ERR_BAD_INDEX = 6     /* an embedding id or a cache page was outside its table (clamped or left out, not trapped on) */
 } ttb_status;
 
 typedef enum { TTB_F32 = 0, TTB_F16 = 1, TTB_BF16 = 2, TTB_I8 = 3 } ttb_dtype;
@@ -387,6 +387,98 @@ int ttb_attention_decode(ttb_ctx* ctx, int dtype, const void* qkv, int64_t B, in
  * 1 <= Lk <= 1024; a head is a multiple of 16 bytes, at most 512. */
 int ttb_context_attention_step(ttb_ctx* ctx, int dtype, const void* q, const void* k, const void* v, const float* mask, int64_t B,
                                int64_t heads, int64_t Lk, int64_t d, float scale, void* probs, void* out);
+
+/* ================= serving over a pool of cache pages =================
+ * No reference counterpart: the reference's decoder concatenates one cache of equally long sequences a step (multi_headed_attention.cpp:207-231), as
+ * ttb_attention_decode does in place. Here every sequence has its own length and its pages lie anywhere in a pool, so that requests come and go, beams share
+ * what they have in common, and prompts are read in chunks.
+ * Lengths, page tables and reference counts are device memory, and nothing below reads them on the host: all of it can be captured into a graph.
+ * At most 1024 sequences (rows of a table) a call. An index that is outside what it indexes is never used: it is clamped or left out, and recorded as
+ * TTB_ERR_BAD_INDEX in the device status word. */
+
+/* Rotary positions: of every head of q[tokens, heads, d] and k[tokens, kv_heads, d] (kv_heads = 0: none) the first rotary_dim elements are turned in pairs, pair i
+ * by the angle positions[t] * freqs[i]: (a, b) -> scale * (a cos - b sin, b cos + a sin). The pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) if interleaved; the
+ * other elements are copied. freqs [rotary_dim / 2] are doubles, radians a position, so that far positions keep their angles; stretching for long contexts is a
+ * matter of freqs and scale. ld*: elements between tokens, a token's heads being d apart. The outputs may be the inputs (same stride) and must not overlap
+ * them otherwise. d % 8 == 0, d <= 512. Rows of a multiple of 16 bytes on 16-byte boundaries, with rotary_dim a multiple of 16 (interleaved: 8), are moved
+ * 16 bytes at a time, others by element. */
+typedef struct ttb_rotary_args {
+  int dtype; /* F32, F16, BF16 */
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t ldq, ldk, ldq_out, ldk_out;
+  int64_t tokens, heads, kv_heads, d, rotary_dim;
+  const int64_t* positions;
+  const double* freqs;
+  int interleaved;
+  float scale;
+} ttb_rotary_args;
+int ttb_rotary(ttb_ctx* ctx, const ttb_rotary_args* args);
+
+/* One layer's keys and values in pages, and whose they are.
+ *   keys, values : [pages, kv_heads, page_tokens, d], page_stride elements between pages (% 8 == 0), 16-byte aligned; F16 or BF16; page_tokens 16, 32, 64, 128 or
+ *                  256; d 64 or 128
+ *   table        : int32 [B, table_width], table_stride between rows: token j of sequence b is in page table[b][j / page_tokens], row j % page_tokens
+ *   cu_seqlens   : int32 [B+1]: sequence b's new tokens are rows [cu[b], cu[b+1]) of the call's q, k, v; rows outside [cu[0], cu[B]) are left alone
+ *   past_lens    : int32 [B]: tokens of sequence b that were cached before: new token i is token past + i */
+typedef struct ttb_paged_kv {
+  void *keys, *values;
+  int64_t page_stride, pages, kv_heads, page_tokens, d;
+  const int32_t* table;
+  int64_t table_stride, table_width;
+  const int32_t *cu_seqlens, *past_lens;
+  int64_t B;
+} ttb_paged_kv;
+/* The rotary positions of ttb_paged_append: k is turned by its tokens' places in their sequences, and so is q[tokens, heads, d] into q_out (heads = 0: none). */
+typedef struct ttb_paged_rotary {
+  const double* freqs;
+  int64_t rotary_dim;
+  int interleaved;
+  float scale;
+  const void* q;
+  void* q_out;
+  int64_t ldq, ldq_out, heads;
+} ttb_paged_rotary;
+/* Files the new tokens' k, v [tokens, kv_heads, d] (ldk, ldv elements between tokens) into their pages, k turned if rotary is not NULL. A token whose page is
+ * not in the pool is not filed. No two rows of the table may list the same page where new tokens go. */
+int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                     const ttb_paged_rotary* rotary);
+
+/* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the cached tokens of t's sequence up to and including its own (causal), or all past + new of them.
+ * The new tokens have been filed (ttb_paged_append). q and out [tokens, heads, d], heads a multiple of kv_heads (query heads h * heads / kv_heads and
+ * following share key head h), ldq / ldo elements between tokens (% 8 == 0), 16-byte aligned; out does not overlap q. scale > 0. What the pages hold behind a
+ * sequence's last token is not looked at; the keys and values of its own tokens are to be finite. A page that is not in the pool is read as page 0. */
+int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const void* q, int64_t ldq, int64_t tokens, int64_t heads, int causal, float scale,
+                        void* out, int64_t ldo);
+
+/* The pages of B sequences: table int32 [B, width] (stride between rows), -1 behind a row's last page; lens int32 [B], the tokens cached; refs int32 [pages], how
+ * many rows list a page (0: it is free). */
+typedef struct ttb_paged_tables {
+  int32_t* table;
+  int64_t stride, B, width;
+  int32_t *lens, *refs;
+  int64_t pages;
+} ttb_paged_tables;
+/* A stack's pages: `planes` (of each layer the keys and the values) of `pages` pages of page_bytes; strides in bytes; everything a multiple of 16. */
+typedef struct ttb_paged_pool {
+  void* base;
+  int64_t planes, plane_stride, pages, page_stride, page_bytes;
+} ttb_paged_pool;
+/* Room for new_tokens[b] more tokens (0: the row is left alone) of every row, before ttb_paged_append: the lowest free pages, in the rows' order. A row whose
+ * last page is begun and listed by other rows too gets a page of its own in its place: copies[i] = (from, to), i < B, in the rows' order, (-1, -1) behind the
+ * last, for ttb_paged_copy, which goes before the next append. (Of rows that are all of a page's holders the last keeps it.) granted[b] = 1, or 0 where the
+ * pages do not suffice: from the first such row on nothing is granted, so that no later row overtakes it; or where the row of the table is too short. lens is left
+ * to the caller, who adds the new tokens when all layers have filed them. */
+int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies);
+/* Row b becomes what row parents[b] was (its pages are shared, not copied), for beams that follow their parents and requests that fork; -1 frees the row: its
+ * length becomes 0. Any number of rows may have the same parent. A parent outside [-1, B) leaves its row as it is. */
+int ttb_paged_fork(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* parents);
+/* Page pairs[i][1] of every plane becomes a copy of page pairs[i][0] (int32 [n, 2] on the device); pairs with a negative entry are left out. A page that is written
+ * may not be in another pair. */
+int ttb_paged_copy(ttb_ctx* ctx, const ttb_paged_pool* pool, const int32_t* pairs, int64_t n);
+/* Moves the used pages to the front of the pool, those behind it into the free ones within it, both in order; table and refs follow. *used (device int32) receives
+ * how many there are. lens is not looked at. */
+int ttb_paged_compact(ttb_ctx* ctx, const ttb_paged_tables* tables, const ttb_paged_pool* pool, int32_t* used);
 
 /* A whole stack of transformer layers over few rows (at most TTB_CHAIN_MAX_ROWS) as one kernel. A request of a few tokens, or
  * one decoding step of a batch, is a chain of some hundred small dependent products; as kernels of their own each costs a launch and a

@@ -51,6 +51,34 @@ class ChainOp(C.Structure):
     _fields_ = [("kind", C.c_int32), ("reserved", C.c_int32), ("u", _U)]
 
 
+class RotaryArgs(C.Structure):
+    """ttb_rotary_args of include/ttb.h."""
+    _fields_ = [("dtype", i32)] + [(n, p) for n in ("q", "k", "q_out", "k_out")] + \
+               [(n, i64) for n in ("ldq", "ldk", "ldq_out", "ldk_out", "tokens", "heads", "kv_heads", "d", "rotary_dim")] + \
+               [("positions", p), ("freqs", p), ("interleaved", i32), ("scale", f32)]
+
+
+class PagedKV(C.Structure):
+    """ttb_paged_kv of include/ttb.h."""
+    _fields_ = [("keys", p), ("values", p)] + [(n, i64) for n in ("page_stride", "pages", "kv_heads", "page_tokens", "d")] + \
+               [("table", p), ("table_stride", i64), ("table_width", i64), ("cu_seqlens", p), ("past_lens", p), ("B", i64)]
+
+
+class PagedRotary(C.Structure):
+    """ttb_paged_rotary of include/ttb.h."""
+    _fields_ = [("freqs", p), ("rotary_dim", i64), ("interleaved", i32), ("scale", f32), ("q", p), ("q_out", p), ("ldq", i64), ("ldq_out", i64), ("heads", i64)]
+
+
+class PagedTables(C.Structure):
+    """ttb_paged_tables of include/ttb.h."""
+    _fields_ = [("table", p), ("stride", i64), ("B", i64), ("width", i64), ("lens", p), ("refs", p), ("pages", i64)]
+
+
+class PagedPool(C.Structure):
+    """ttb_paged_pool of include/ttb.h."""
+    _fields_ = [("base", p)] + [(n, i64) for n in ("planes", "plane_stride", "pages", "page_stride", "page_bytes")]
+
+
 CHAIN_WORKSPACE = 256
 CHAIN_KEYS_ROWS, CHAIN_KEYS_CACHE, CHAIN_KEYS_MEMORY = 0, 1, 2
 
@@ -82,6 +110,13 @@ SIGNATURES = {
     "ttb_kv_cache_append": (i32, [p, i32, p, i64, i64, i64, i64, p, p, i64]),
     "ttb_context_attention_step": (i32, [p, i32, p, p, p, p, i64, i64, i64, i64, f32, p, p]),
     "ttb_attention_decode": (i32, [p, i32, p, i64, i64, i64, i64, p, p, i64, f32, p]),
+    "ttb_rotary": (i32, [p, C.POINTER(RotaryArgs)]),
+    "ttb_paged_append": (i32, [p, i32, C.POINTER(PagedKV), i64, p, i64, p, i64, C.POINTER(PagedRotary)]),
+    "ttb_paged_attention": (i32, [p, i32, C.POINTER(PagedKV), p, i64, i64, i64, i32, f32, p, i64]),
+    "ttb_paged_reserve": (i32, [p, C.POINTER(PagedTables), p, i64, p, p]),
+    "ttb_paged_fork": (i32, [p, C.POINTER(PagedTables), p]),
+    "ttb_paged_copy": (i32, [p, C.POINTER(PagedPool), p, i64]),
+    "ttb_paged_compact": (i32, [p, C.POINTER(PagedTables), C.POINTER(PagedPool), p]),
     "ttb_chain_forward": (i32, [p, i32, C.POINTER(ChainOp), i32, p]),
     "ttb_chain_forward_flow": (i32, [p, i32, C.POINTER(ChainOp), i32, p, i64]),
     "ttb_token_position_embedding": (i32, [p, i32, p, p, p, p, i64, i64, i64, i64]),
@@ -213,6 +248,38 @@ class Context:
         for name, value in fields.items():
             setattr(a, name, value.data_ptr() if hasattr(value, "data_ptr") else value)
         self.check(lib().ttb_linear_split(self.h, C.byref(a)))
+
+    @staticmethod
+    def _filled(block, fields):
+        for name, value in fields.items():
+            setattr(block, name, value.data_ptr() if hasattr(value, "data_ptr") else value)
+        return block
+
+    def rotary(self, **fields):
+        """ttb_rotary with the argument block filled by the fields' names; tensors are passed as their pointers, here and below."""
+        self.check(lib().ttb_rotary(self.h, C.byref(self._filled(RotaryArgs(), fields))))
+
+    def paged_append(self, dtype, kv, tokens, k, ldk, v, ldv, rotary=None):
+        """ttb_paged_append; kv and rotary: dicts of their blocks' fields."""
+        block = C.byref(self._filled(PagedRotary(), rotary)) if rotary is not None else None
+        self.check(lib().ttb_paged_append(self.h, dtype, C.byref(self._filled(PagedKV(), kv)), tokens, p(k.data_ptr()), ldk, p(v.data_ptr()), ldv, block))
+
+    def paged_attention(self, dtype, kv, q, ldq, tokens, heads, causal, scale, out, ldo):
+        self.check(lib().ttb_paged_attention(self.h, dtype, C.byref(self._filled(PagedKV(), kv)), p(q.data_ptr()), ldq, tokens, heads, causal, scale,
+                                             p(out.data_ptr()), ldo))
+
+    def paged_reserve(self, tables, new_tokens, page_tokens, granted, copies):
+        self.check(lib().ttb_paged_reserve(self.h, C.byref(self._filled(PagedTables(), tables)), p(new_tokens.data_ptr()), page_tokens, p(granted.data_ptr()),
+                                           p(copies.data_ptr())))
+
+    def paged_fork(self, tables, parents):
+        self.check(lib().ttb_paged_fork(self.h, C.byref(self._filled(PagedTables(), tables)), p(parents.data_ptr())))
+
+    def paged_copy(self, pool, pairs, n):
+        self.check(lib().ttb_paged_copy(self.h, C.byref(self._filled(PagedPool(), pool)), p(pairs.data_ptr()), n))
+
+    def paged_compact(self, tables, pool, used):
+        self.check(lib().ttb_paged_compact(self.h, C.byref(self._filled(PagedTables(), tables)), C.byref(self._filled(PagedPool(), pool)), p(used.data_ptr())))
 
     @staticmethod
     def _chain_block(ops):

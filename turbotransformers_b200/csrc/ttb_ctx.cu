@@ -115,7 +115,7 @@ extern "C" int ttb_device_status(ttb_ctx* c) {
   TTB_CUDA(c, cudaStreamSynchronize(c->stream));
   int s = *c->h_status;
   if (s == TTB_ERR_DEVICE_WAIT) return fail(c, s, "a bounded device-side wait expired inside a kernel");
-  if (s == TTB_ERR_BAD_INDEX) return fail(c, s, "an embedding id was outside its table (clamped)");
+  if (s == TTB_ERR_BAD_INDEX) return fail(c, s, "an embedding id or a cache page was outside its table (clamped or left out)");
   if (s != 0) return fail(c, TTB_ERR_CUDA, "device status word holds %d", s);
   return TTB_OK;
 }

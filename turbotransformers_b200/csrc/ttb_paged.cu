@@ -1,0 +1,592 @@
+// Rotary positions, the new tokens of ragged sequences filed into cache pages, and the pages' own maintenance.
+#include <algorithm>
+#include <climits>
+
+#include "ttb_paged.cuh"
+
+using namespace ttb;
+using namespace ttb::paged;
+
+namespace {
+
+// ---- rotary positions -------------------------------------------------------------------------------------------------
+// A pair (a, b) of a head becomes scale * (a cos r - b sin r, b cos r + a sin r) with r = position * frequency: pairs (i, i + n/2) of the first n elements, or
+// neighbours. Bound by reading and writing the rows once. A block takes a few tokens: their sines and cosines are made once for all heads and kept in shared
+// memory. The angle is a product of doubles in turns, of which the whole ones are dropped before it is rounded to fp32: a position of a
+// million times a frequency in fp32 would be off by a tenth of a radian. With a pool of pages, k is turned on its way into its page and v copied beside it: a pass
+// of its own over both, and a launch, saved.
+constexpr int kRotaryThreads = 256;
+constexpr int kRotaryTokens = 8;  // of a block, at most
+
+struct RotaryParams {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  long long ldq, ldk, ldv, ldq_out, ldk_out;
+  int tokens, heads, kv_heads, d, half, interleaved, block_tokens;
+  float scale;
+  const int64_t* positions;
+  const double* freqs;
+  Sequences s;              // PAGED
+  void *keys, *values;
+  long long page_stride;
+};
+
+// Which sequence row t belongs to, by the whole warp: the entries of cu that are at most t, counted in two looks of a lane each.
+__device__ __forceinline__ int sequence_at(const Sequences& s, int t, int lane) {
+  const int step = (s.B + 32) / 32;  // at most 33 for kMaxSequences
+  const int at = lane * step;
+  const int before = __popc(__ballot_sync(0xffffffffu, at <= s.B && s.cu[min(at, s.B)] <= t));
+  if (before == 0) return -1;
+  const int lo = (before - 1) * step, i = lo + 1 + lane;
+  return lo + __popc(__ballot_sync(0xffffffffu, i < lo + step && i <= s.B && s.cu[min(i, s.B)] <= t));
+}
+
+// One unit of a head, in place or not: WIDE, eight pairs (halves) or four (neighbours), or eight elements that are not turned; else a pair or an element.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void turn_unit(const T* src, T* dst, int unit, int half, int interleaved, const float2* cs) {
+  if (WIDE) {
+    if (interleaved) {
+      Vec8<T> x;
+      x.load(src + unit * 8);
+      if (unit * 4 < half) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 c = cs[unit * 4 + e];
+          const float a = x.v[2 * e], b = x.v[2 * e + 1];
+          x.v[2 * e] = a * c.x - b * c.y;
+          x.v[2 * e + 1] = b * c.x + a * c.y;
+        }
+      }
+      x.store(dst + unit * 8);
+    } else if (unit * 8 < half) {
+      Vec8<T> x, y;
+      x.load(src + unit * 8);
+      y.load(src + half + unit * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 c = cs[unit * 8 + e];
+        const float a = x.v[e], b = y.v[e];
+        x.v[e] = a * c.x - b * c.y;
+        y.v[e] = b * c.x + a * c.y;
+      }
+      x.store(dst + unit * 8);
+      y.store(dst + half + unit * 8);
+    } else {
+      Vec8<T> x;
+      x.load(src + half + unit * 8);
+      x.store(dst + half + unit * 8);
+    }
+  } else if (unit < half) {
+    const int i = interleaved ? 2 * unit : unit, j = interleaved ? 2 * unit + 1 : unit + half;
+    const float a = to_f(src[i]), b = to_f(src[j]);
+    const float2 c = cs[unit];
+    dst[i] = from_f<T>(a * c.x - b * c.y);
+    dst[j] = from_f<T>(b * c.x + a * c.y);
+  } else {
+    dst[half + unit] = src[half + unit];
+  }
+}
+
+template <typename T, bool WIDE, bool PAGED>
+__global__ void __launch_bounds__(kRotaryThreads)
+rotary_kernel(const RotaryParams p) {
+  extern __shared__ float2 cs[];  // [block_tokens][half]
+  __shared__ double s_pos[kRotaryTokens];
+  __shared__ long long s_page[kRotaryTokens];  // PAGED: the token's first element of the pools, -1: it has no place
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int t0 = blockIdx.x * p.block_tokens, n = min(p.block_tokens, p.tokens - t0);
+  for (int i = PAGED ? warp : tid; i < n; i += PAGED ? kRotaryThreads / 32 : kRotaryThreads) {
+    const int t = t0 + i;
+    if (!PAGED) {
+      s_pos[i] = (double)p.positions[t];
+      continue;
+    }
+    const int b = sequence_at(p.s, t, lane);
+    bool bad = false, mine = false;
+    long long place = -1;
+    int at = 0;
+    if (b >= 0 && b < p.s.B) {
+      const Sequence q = sequence_of(p.s, b, &bad);
+      mine = t >= q.tok0 && t < q.tok0 + q.n;
+      at = q.past + t - q.tok0;
+      if (mine && at < p.s.cap) {
+        bool bad_page;
+        const int page = page_of(p.s, b, at, &bad_page);
+        bad |= bad_page;
+        if (!bad_page) place = (long long)page * p.page_stride + (long long)(at & ((1 << p.s.page_shift) - 1)) * p.d;
+      }
+    }
+    if (lane == 0) {
+      if (bad) bad_index(p.s.status);
+      s_pos[i] = mine ? (double)at : -1.0;
+      s_page[i] = place;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < n * p.half; i += kRotaryThreads) {
+    const double turns = s_pos[i / p.half] * p.freqs[i % p.half] * 0.15915494309189533577;  // 1 / (2 pi)
+    float s, c;
+    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+    cs[i] = make_float2(c * p.scale, s * p.scale);
+  }
+  __syncthreads();
+  // units of a head, of a token's queries, its keys, and (PAGED) its values
+  const int wide = p.interleaved ? p.d / 8 : (p.d - p.half) / 8;
+  const int per = WIDE ? wide : p.d - p.half, qn = p.heads * per, kn = p.kv_heads * per, vn = PAGED ? p.kv_heads * p.d / (WIDE ? 8 : 1) : 0;
+  const int each = qn + kn + vn;
+  for (int idx = tid; idx < n * each; idx += kRotaryThreads) {
+    const int i = idx / each, u = idx - i * each, t = t0 + i;
+    const float2* c = cs + i * p.half;
+    if (u < qn) {
+      if (PAGED && s_pos[i] < 0) continue;
+      const int h = u / per;
+      turn_unit<T, WIDE>(static_cast<const T*>(p.q) + t * p.ldq + h * p.d, static_cast<T*>(p.q_out) + t * p.ldq_out + h * p.d, u - h * per, p.half, p.interleaved, c);
+    } else if (u < qn + kn) {
+      if (PAGED && s_page[i] < 0) continue;
+      const int h = (u - qn) / per;
+      T* dst = PAGED ? static_cast<T*>(p.keys) + s_page[i] + ((long long)h << p.s.page_shift) * p.d : static_cast<T*>(p.k_out) + t * p.ldk_out + h * p.d;
+      turn_unit<T, WIDE>(static_cast<const T*>(p.k) + t * p.ldk + h * p.d, dst, u - qn - h * per, p.half, p.interleaved, c);
+    } else if (PAGED) {
+      if (s_page[i] < 0) continue;
+      const int w = WIDE ? p.d / 8 : p.d, h = (u - qn - kn) / w, e = (u - qn - kn - h * w) * (p.d / w);
+      const T* src = static_cast<const T*>(p.v) + t * p.ldv + h * p.d + e;
+      T* dst = static_cast<T*>(p.values) + s_page[i] + ((long long)h << p.s.page_shift) * p.d + e;
+      if (WIDE) {
+        Vec8<T> x;
+        x.load(src);
+        x.store(dst);
+      } else {
+        *dst = *src;
+      }
+    }
+  }
+}
+
+template <typename T, bool PAGED>
+int launch_rotary(ttb_ctx* ctx, RotaryParams& p, const char* what) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                       reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out);
+  const bool wide = (at & 15) == 0 && ((p.ldq | p.ldk | p.ldv | p.ldq_out | p.ldk_out) * (int)sizeof(T)) % 16 == 0 && p.half % (p.interleaved ? 4 : 8) == 0;
+  // tokens of a block: enough for every thread to have some units, few enough for the tokens to reach all SMs
+  const int units = (p.heads + (PAGED ? 2 : 1) * p.kv_heads) * p.d / 16;
+  p.block_tokens = std::max(1, std::min(std::min(kRotaryTokens, 4 * kRotaryThreads / std::max(1, units)), p.tokens / (4 * ctx->sm_count)));
+  const dim3 grid((unsigned)((p.tokens + p.block_tokens - 1) / p.block_tokens));
+  const size_t smem = (size_t)p.block_tokens * p.half * sizeof(float2);
+  if (wide) launch_pdl(rotary_kernel<T, true, PAGED>, grid, dim3(kRotaryThreads), smem, ctx->stream, p);
+  else launch_pdl(rotary_kernel<T, false, PAGED>, grid, dim3(kRotaryThreads), smem, ctx->stream, p);
+  return launched(ctx, what);
+}
+
+// ---- page maintenance ---------------------------------------------------------------------------------------------------
+// The page table, the lengths and the reference counts stay on the device, and so do the decisions: a step of a captured graph forks beams and takes pages
+// without the host. Every choice goes by rows' and pages' order, so that it is the same on every run. All are bound by latency but the copies.
+constexpr int kManageThreads = 1024;
+constexpr int kScanRefs = 16;  // reference counts a thread looks at in one round
+
+// Exclusive prefix sum over the block; *total receives the sum. `scratch` holds 33 ints.
+__device__ __forceinline__ int block_scan(int v, int* scratch, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  __syncthreads();  // the scratch's last readers are through
+  if (lane == 31) scratch[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int w = lane < warps ? scratch[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += x;
+    }
+    scratch[lane] = w;
+    if (lane == 31) scratch[32] = w;
+  }
+  __syncthreads();
+  *total = scratch[32];
+  return incl - v + (warp ? scratch[warp - 1] : 0);
+}
+
+struct Tables {
+  int32_t* table;
+  long long stride;
+  int B, width, pages;
+  int32_t *lens, *refs;
+  int* status;
+};
+
+// Pages for new[b] more tokens of every row (see ttb.h for the rules). One block; thread b decides for row b, then a warp a row fills the table in.
+// free_list [pages], sharers [pages], keeper [pages]: scratch, not initialised.
+__global__ void __launch_bounds__(kManageThreads, 1)
+paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page_tokens, int32_t* granted, int32_t* copies, int* free_list, int* sharers,
+                     int* keeper) {
+  __shared__ int scratch[33];
+  __shared__ int s_first[kMaxSequences], s_want[kMaxSequences], s_base[kMaxSequences];
+  pdl_trigger();
+  pdl_wait();
+  const int b = threadIdx.x;
+  int len = 0, add = 0, have = 0, want = 0, last = -1, last_refs = 0;
+  bool fits = false, open = false;
+  if (b < t.B) {
+    len = t.lens[b];
+    add = fresh[b];
+    const long long cap = (long long)t.width * page_tokens;
+    fits = len >= 0 && add >= 0 && (long long)len + add <= cap;
+    if (len < 0 || add < 0 || len > cap) bad_index(t.status);
+    if (fits) {
+      have = (len + page_tokens - 1) / page_tokens;
+      want = (len + add + page_tokens - 1) / page_tokens;
+      if (add > 0 && len % page_tokens != 0) {
+        last = t.table[b * t.stride + have - 1];
+        open = last >= 0 && last < t.pages;
+        if (!open) bad_index(t.status);
+      }
+    }
+    if (open) {
+      last_refs = t.refs[last];
+      sharers[last] = 0;
+      keeper[last] = -1;
+    }
+  }
+  __threadfence_block();
+  __syncthreads();
+  if (open) {
+    atomicAdd(sharers + last, 1);
+    atomicMax(keeper + last, b);
+  }
+  __threadfence_block();
+  __syncthreads();
+  // rows that are all of a page's holders: the last of them keeps it
+  bool copy = open && last_refs > 1 && !(__ldcg(sharers + last) == last_refs && __ldcg(keeper + last) == b);
+  const bool writes = add > 0;
+  const int need = writes && fits ? want - have + (copy ? 1 : 0) : 0;
+  int total, found = 0;
+  const int before = block_scan(need, scratch, &total);
+  // the lowest free pages, as many as are needed
+  for (int p0 = 0; p0 < t.pages && found < total; p0 += kManageThreads * kScanRefs) {
+    uint32_t free = 0;
+    const int mine = p0 + (int)threadIdx.x * kScanRefs;
+#pragma unroll
+    for (int i = 0; i < kScanRefs; ++i)
+      if (mine + i < t.pages && t.refs[mine + i] <= 0) free |= 1u << i;
+    int round;
+    int at = found + block_scan(__popc(free), scratch, &round);
+    for (; free && at < total; free &= free - 1) free_list[at++] = mine + __ffs(free) - 1;
+    found += round;
+  }
+  __threadfence_block();
+  __syncthreads();
+  const bool ok = !writes || (fits && (long long)before + need <= found);
+  copy = copy && ok;
+  int n_copies;
+  const int c = block_scan(copy ? 1 : 0, scratch, &n_copies);
+  if (b < t.B) {
+    granted[b] = ok;
+    s_first[b] = copy ? have - 1 : have;
+    s_want[b] = ok && writes ? want : 0;
+    s_base[b] = before;
+    if (copy) {
+      copies[2 * c] = last;
+      copies[2 * c + 1] = free_list[before];
+      atomicSub(t.refs + last, 1);
+    }
+    if (b >= n_copies) copies[2 * b] = copies[2 * b + 1] = -1;
+  }
+  __syncthreads();
+  for (int row = threadIdx.x >> 5; row < t.B; row += kManageThreads / 32)
+    for (int col = s_first[row] + (threadIdx.x & 31); col < s_want[row]; col += 32) {
+      const int page = free_list[s_base[row] + col - s_first[row]];
+      t.table[row * t.stride + col] = page;
+      t.refs[page] = 1;
+    }
+}
+
+// Row b becomes what row parents[b] was. A block takes some columns of all rows: it has read them all before it writes the first, and no other block touches
+// them. Reference counts are sums, which no order changes.
+constexpr int kForkColumns = 16;
+__global__ void __launch_bounds__(256)
+paged_fork_kernel(const Tables t, const int32_t* __restrict__ parents) {
+  extern __shared__ int32_t old[];  // [B][kForkColumns], then the lengths
+  pdl_trigger();
+  pdl_wait();
+  const int c0 = blockIdx.x * kForkColumns, n = min(kForkColumns, t.width - c0);
+  int32_t* s_lens = old + t.B * kForkColumns;
+  for (int i = threadIdx.x; i < t.B * kForkColumns; i += blockDim.x)
+    if (i % kForkColumns < n) old[i] = t.table[i / kForkColumns * t.stride + c0 + i % kForkColumns];
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < t.B; b += blockDim.x) s_lens[b] = t.lens[b];
+  __syncthreads();
+  auto parent_of = [&](int b) {
+    const int p = parents[b];
+    if (p < -1 || p >= t.B) {
+      bad_index(t.status);
+      return b;
+    }
+    return p;
+  };
+  for (int i = threadIdx.x; i < t.B * kForkColumns; i += blockDim.x) {
+    const int b = i / kForkColumns, c = i % kForkColumns;
+    if (c >= n) continue;
+    const int parent = parent_of(b);
+    const int before = old[i], after = parent < 0 ? -1 : old[parent * kForkColumns + c];
+    if (after == before) continue;
+    if (after >= t.pages || before >= t.pages) bad_index(t.status);
+    if (after >= 0 && after < t.pages) atomicAdd(t.refs + after, 1);
+    if (before >= 0 && before < t.pages) atomicSub(t.refs + before, 1);
+    t.table[b * t.stride + c0 + c] = after;
+  }
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < t.B; b += blockDim.x) {
+      const int parent = parent_of(b);
+      t.lens[b] = parent < 0 ? 0 : s_lens[parent];
+    }
+}
+
+// Page pairs[i][1] of every plane becomes a copy of page pairs[i][0]. A block copies a page of one plane at a time; pairs with a negative entry are left out.
+constexpr int kCopyThreads = 256;
+constexpr int kCopyDepth = 8;  // 16-byte loads a thread has in flight
+__global__ void __launch_bounds__(kCopyThreads)
+paged_copy_kernel(uint4* pool, int planes, long long plane_stride, int page_chunks, long long page_stride, int pages, const int32_t* pairs, int n_pairs, const int* count,
+                  int* status) {
+  pdl_trigger();
+  pdl_wait();
+  const long long n = (long long)(count ? min(*count, n_pairs) : n_pairs) * planes;
+  for (long long w = blockIdx.x; w < n; w += gridDim.x) {
+    const int pair = (int)(w / planes), plane = (int)(w - (long long)pair * planes);
+    const int from = pairs[2 * pair], to = pairs[2 * pair + 1];
+    if (from < 0 || to < 0) continue;
+    if (from >= pages || to >= pages) {
+      bad_index(status);
+      continue;
+    }
+    const uint4* src = pool + plane * plane_stride + from * page_stride;
+    uint4* dst = pool + plane * plane_stride + to * page_stride;
+    for (int i0 = threadIdx.x; i0 < page_chunks; i0 += kCopyThreads * kCopyDepth) {
+      uint4 v[kCopyDepth];
+#pragma unroll
+      for (int k = 0; k < kCopyDepth; ++k)
+        if (i0 + k * kCopyThreads < page_chunks) v[k] = src[i0 + k * kCopyThreads];
+#pragma unroll
+      for (int k = 0; k < kCopyDepth; ++k)
+        if (i0 + k * kCopyThreads < page_chunks) dst[i0 + k * kCopyThreads] = v[k];
+    }
+  }
+}
+
+// Which pages move where: the used ones behind the front (as many as are used), in order, into the free ones within it, in order. One block.
+// to [pages]: where each page is afterwards; pairs [pages / 2][2]; n_moves.
+__global__ void __launch_bounds__(kManageThreads, 1)
+paged_compact_kernel(int32_t* refs, int pages, int32_t* used, int32_t* to, int32_t* pairs, int* n_moves) {
+  __shared__ int scratch[33];
+  pdl_trigger();
+  pdl_wait();
+  int live = 0, front;
+  for (int p = threadIdx.x; p < pages; p += kManageThreads) live += refs[p] > 0;
+  block_scan(live, scratch, &front);
+  int outs = 0, holes = 0;
+  for (int p0 = 0; p0 < pages; p0 += kManageThreads) {
+    const int p = p0 + (int)threadIdx.x;
+    const bool in_use = p < pages && refs[p] > 0, out = in_use && p >= front, hole = p < front && !in_use;
+    int total;
+    const int at = block_scan((out ? 1 << 16 : 0) + (hole ? 1 : 0), scratch, &total);  // both at once: at most 1024 of each in a round
+    if (out) pairs[2 * (outs + (at >> 16))] = p;
+    if (hole) pairs[2 * (holes + (at & 0xffff)) + 1] = p;
+    if (p < pages) to[p] = p;
+    outs += total >> 16;
+    holes += total & 0xffff;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int i = threadIdx.x; i < outs; i += kManageThreads) {
+    const int from = pairs[2 * i], hole = pairs[2 * i + 1];
+    to[from] = hole;
+    refs[hole] = refs[from];
+    refs[from] = 0;
+  }
+  if (threadIdx.x == 0) {
+    *used = front;
+    *n_moves = outs;
+  }
+}
+
+__global__ void __launch_bounds__(256)
+paged_remap_kernel(const Tables t, const int32_t* __restrict__ to) {
+  pdl_trigger();
+  pdl_wait();
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)t.B * t.width; i += (long long)gridDim.x * 256) {
+    int32_t* e = t.table + i / t.width * t.stride + i % t.width;
+    const int page = *e;
+    if (page >= t.pages) bad_index(t.status);
+    else if (page >= 0) *e = to[page];
+  }
+}
+
+int check_tables(ttb_ctx* ctx, const char* what, const ttb_paged_tables* a, Tables* t) {
+  TTB_REQUIRE(ctx, a, "%s: null arguments", what);
+  TTB_REQUIRE(ctx, a->refs && (a->table || a->B == 0), "%s: null pointer", what);
+  TTB_REQUIRE(ctx, a->B >= 0 && a->B <= kMaxSequences, "%s: at most %d rows", what, kMaxSequences);
+  TTB_REQUIRE(ctx, a->width > 0 && a->width < (1ll << 30) && a->stride >= a->width, "%s: bad table width", what);
+  TTB_REQUIRE(ctx, a->pages > 0 && a->pages < (1ll << 30), "%s: bad number of pages", what);
+  *t = Tables{a->table, a->stride, (int)a->B, (int)a->width, (int)a->pages, a->lens, a->refs, ctx->d_status};
+  return TTB_OK;
+}
+
+int check_pool(ttb_ctx* ctx, const char* what, const ttb_paged_pool* a) {
+  TTB_REQUIRE(ctx, a && a->base, "%s: null pool", what);
+  TTB_REQUIRE(ctx, a->planes > 0 && a->planes < (1ll << 20) && a->pages > 0 && a->pages < (1ll << 30) && a->page_bytes > 0 && a->page_bytes < (1ll << 31),
+              "%s: bad pool shape", what);
+  TTB_REQUIRE(ctx, a->page_stride >= a->page_bytes && (a->planes == 1 || a->plane_stride >= (a->pages - 1) * a->page_stride + a->page_bytes),
+              "%s: the pool's pages overlap", what);
+  TTB_REQUIRE(ctx, ((reinterpret_cast<uintptr_t>(a->base) | (uintptr_t)a->page_bytes | (uintptr_t)a->page_stride | (uintptr_t)a->plane_stride) & 15) == 0,
+              "%s: the pool, its pages and its planes must be multiples of 16 bytes", what);
+  return TTB_OK;
+}
+
+int launch_copy(ttb_ctx* ctx, const ttb_paged_pool* a, const int32_t* pairs, int64_t n, const int* count) {
+  const unsigned grid = (unsigned)std::min<int64_t>(n * a->planes, (int64_t)ctx->sm_count * 8);
+  launch_pdl(paged_copy_kernel, dim3(grid), dim3(kCopyThreads), 0, ctx->stream, static_cast<uint4*>(a->base), (int)a->planes, (long long)(a->plane_stride / 16),
+             (int)(a->page_bytes / 16), (long long)(a->page_stride / 16), (int)a->pages, pairs, (int)n, count, ctx->d_status);
+  return launched(ctx, "paged_copy");
+}
+
+}  // namespace
+
+extern "C" int ttb_rotary(ttb_ctx* ctx, const ttb_rotary_args* a) {
+  if (!ctx) return TTB_ERR_INVALID;
+  TTB_REQUIRE(ctx, a, "rotary: null arguments");
+  TTB_REQUIRE(ctx, a->dtype == TTB_F32 || a->dtype == TTB_F16 || a->dtype == TTB_BF16, "rotary: dtype must be F32, F16 or BF16");
+  TTB_REQUIRE(ctx, a->tokens >= 0 && a->tokens < (1ll << 29) && a->heads > 0 && a->heads <= 65535 && a->kv_heads >= 0 && a->kv_heads <= 65535, "rotary: bad shape");
+  TTB_REQUIRE(ctx, a->d > 0 && a->d % 8 == 0 && a->d <= 512, "rotary: the head size must be a multiple of 8, at most 512");
+  TTB_REQUIRE(ctx, a->rotary_dim > 0 && a->rotary_dim % 2 == 0 && a->rotary_dim <= a->d, "rotary: an even number of a head's elements is turned");
+  if (a->tokens == 0) return TTB_OK;
+  TTB_REQUIRE(ctx, (a->kv_heads == 0) == (a->k == nullptr), "rotary: keys without key heads, or key heads without keys");
+  TTB_REQUIRE(ctx, a->q && a->q_out && (a->kv_heads == 0 || a->k_out) && a->positions && a->freqs, "rotary: null pointer");
+  const int64_t nq = a->heads * a->d, nk = a->kv_heads * a->d;
+  TTB_REQUIRE(ctx, a->ldq >= nq && a->ldq_out >= nq && (nk == 0 || (a->ldk >= nk && a->ldk_out >= nk)), "rotary: rows overlap");
+  DeviceGuard g(ctx->device);
+  RotaryParams p = {};
+  p.q = a->q; p.q_out = a->q_out; p.ldq = a->ldq; p.ldq_out = a->ldq_out;
+  if (nk) { p.k = a->k; p.k_out = a->k_out; p.ldk = a->ldk; p.ldk_out = a->ldk_out; }
+  p.tokens = (int)a->tokens; p.heads = (int)a->heads; p.kv_heads = (int)a->kv_heads; p.d = (int)a->d;
+  p.half = (int)(a->rotary_dim / 2);
+  p.interleaved = a->interleaved != 0;
+  p.scale = a->scale;
+  p.positions = a->positions;
+  p.freqs = a->freqs;
+  if (a->dtype == TTB_F32) return launch_rotary<float, false>(ctx, p, "rotary");
+  if (a->dtype == TTB_F16) return launch_rotary<__half, false>(ctx, p, "rotary");
+  return launch_rotary<__nv_bfloat16, false>(ctx, p, "rotary");
+}
+
+extern "C" int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                const ttb_paged_rotary* r) {
+  if (!ctx) return TTB_ERR_INVALID;
+  RotaryParams p = {};
+  const int bad = check_kv(ctx, "paged_append", dtype, kv, tokens, &p.s);
+  if (bad) return bad;
+  const int64_t n = kv->kv_heads * kv->d;
+  p.d = (int)kv->d;
+  p.kv_heads = (int)kv->kv_heads;
+  if (r) {
+    TTB_REQUIRE(ctx, r->freqs && r->rotary_dim > 0 && r->rotary_dim % 2 == 0 && r->rotary_dim <= kv->d,
+                "paged_append: an even number of a head's elements is turned");
+    TTB_REQUIRE(ctx, r->heads >= 0 && r->heads <= 65535, "paged_append: bad number of query heads");
+    TTB_REQUIRE(ctx, tokens == 0 || ((r->heads == 0) == (r->q == nullptr) && (r->heads == 0) == (r->q_out == nullptr)),
+                "paged_append: queries without heads, or heads without queries");
+    TTB_REQUIRE(ctx, r->heads == 0 || (r->ldq >= r->heads * kv->d && r->ldq_out >= r->heads * kv->d), "paged_append: rows overlap");
+    p.half = (int)(r->rotary_dim / 2);
+    p.interleaved = r->interleaved != 0;
+    p.scale = r->scale;
+    p.freqs = r->freqs;
+    p.heads = (int)r->heads;
+    if (p.heads) { p.q = r->q; p.q_out = r->q_out; p.ldq = r->ldq; p.ldq_out = r->ldq_out; }
+  }
+  if (tokens == 0 || kv->B == 0) return TTB_OK;
+  TTB_REQUIRE(ctx, k && v, "paged_append: null pointer");
+  TTB_REQUIRE(ctx, ldk >= n && ldv >= n, "paged_append: rows overlap");
+  DeviceGuard g(ctx->device);
+  p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
+  p.keys = kv->keys; p.values = kv->values; p.page_stride = kv->page_stride;
+  p.tokens = (int)tokens;
+  return dtype == TTB_F16 ? launch_rotary<__half, true>(ctx, p, "paged_append") : launch_rotary<__nv_bfloat16, true>(ctx, p, "paged_append");
+}
+
+extern "C" int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* a, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies) {
+  if (!ctx) return TTB_ERR_INVALID;
+  Tables t;
+  const int bad = check_tables(ctx, "paged_reserve", a, &t);
+  if (bad) return bad;
+  TTB_REQUIRE(ctx, page_tokens > 0 && page_tokens <= (1ll << 20) && page_tokens * a->width <= (1ll << 30), "paged_reserve: bad page size");
+  if (a->B == 0) return TTB_OK;
+  TTB_REQUIRE(ctx, a->lens && new_tokens && granted && copies, "paged_reserve: null pointer");
+  DeviceGuard g(ctx->device);
+  void* ws = nullptr;
+  int s = ttb_alloc(ctx, (size_t)a->pages * 3 * sizeof(int), "paged_reserve/scratch", &ws);
+  if (s) return s;
+  int* w = static_cast<int*>(ws);
+  launch_pdl(paged_reserve_kernel, dim3(1), dim3(kManageThreads), 0, ctx->stream, t, new_tokens, (int)page_tokens, granted, copies, w, w + a->pages, w + 2 * a->pages);
+  s = launched(ctx, "paged_reserve");
+  const int f = ttb_free(ctx, ws, "paged_reserve/scratch");
+  return s ? s : f;
+}
+
+extern "C" int ttb_paged_fork(ttb_ctx* ctx, const ttb_paged_tables* a, const int32_t* parents) {
+  if (!ctx) return TTB_ERR_INVALID;
+  Tables t;
+  const int bad = check_tables(ctx, "paged_fork", a, &t);
+  if (bad) return bad;
+  if (a->B == 0) return TTB_OK;
+  TTB_REQUIRE(ctx, a->lens && parents, "paged_fork: null pointer");
+  DeviceGuard g(ctx->device);
+  const size_t smem = (size_t)a->B * (kForkColumns + 1) * sizeof(int32_t);
+  static bool configured[64] = {};
+  const int dev = ctx->device < 64 ? ctx->device : 63;
+  if (!configured[dev]) {
+    TTB_CUDA(ctx, cudaFuncSetAttribute(paged_fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSequences * (kForkColumns + 1) * 4));
+    configured[dev] = true;
+  }
+  launch_pdl(paged_fork_kernel, dim3((unsigned)((a->width + kForkColumns - 1) / kForkColumns)), dim3(256), smem, ctx->stream, t, parents);
+  return launched(ctx, "paged_fork");
+}
+
+extern "C" int ttb_paged_copy(ttb_ctx* ctx, const ttb_paged_pool* pool, const int32_t* pairs, int64_t n) {
+  if (!ctx) return TTB_ERR_INVALID;
+  const int bad = check_pool(ctx, "paged_copy", pool);
+  if (bad) return bad;
+  TTB_REQUIRE(ctx, n >= 0 && n < (1ll << 30), "paged_copy: bad number of pairs");
+  if (n == 0) return TTB_OK;
+  TTB_REQUIRE(ctx, pairs, "paged_copy: null pointer");
+  DeviceGuard g(ctx->device);
+  return launch_copy(ctx, pool, pairs, n, nullptr);
+}
+
+extern "C" int ttb_paged_compact(ttb_ctx* ctx, const ttb_paged_tables* a, const ttb_paged_pool* pool, int32_t* used) {
+  if (!ctx) return TTB_ERR_INVALID;
+  Tables t;
+  int s = check_tables(ctx, "paged_compact", a, &t);
+  if (s) return s;
+  s = check_pool(ctx, "paged_compact", pool);
+  if (s) return s;
+  TTB_REQUIRE(ctx, pool->pages == a->pages, "paged_compact: the pool and the reference counts differ in pages");
+  TTB_REQUIRE(ctx, used, "paged_compact: null pointer");
+  DeviceGuard g(ctx->device);
+  void* ws = nullptr;
+  s = ttb_alloc(ctx, ((size_t)a->pages * 2 + 3) * sizeof(int32_t), "paged_compact/scratch", &ws);
+  if (s) return s;
+  int32_t *to = static_cast<int32_t*>(ws), *pairs = to + a->pages, *moves = pairs + a->pages + 2;
+  launch_pdl(paged_compact_kernel, dim3(1), dim3(kManageThreads), 0, ctx->stream, a->refs, (int)a->pages, used, to, pairs, moves);
+  s = launched(ctx, "paged_compact");
+  if (!s && a->B > 0) {
+    const int64_t n = a->B * a->width;
+    launch_pdl(paged_remap_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)ctx->sm_count * 8)), dim3(256), 0, ctx->stream, t, to);
+    s = launched(ctx, "paged_remap");
+  }
+  if (!s && a->pages > 1) s = launch_copy(ctx, pool, pairs, a->pages / 2, moves);
+  const int f = ttb_free(ctx, ws, "paged_compact/scratch");
+  return s ? s : f;
+}

@@ -9,6 +9,8 @@ from .modeling_smart_pad import (MultiHeadedAttentionSmartBatch, BertLayerSmartB
 from .modeling_distillbert import DistillBertAttention, DistrillFFN, DistrillTransformerBlock, DistrillTransformer, DistilBertModel
 from .modeling_roberta import RobertaModel
 from .modeling_albert import AlbertAttention, AlbertLayer, AlbertLayerGroup, AlbertTransformer, AlbertModel
+from .paged import (rotary, paged_append, paged_attention, paged_reserve, paged_fork, paged_copy, paged_compact, RotaryEmbedding,
+                    PagedKVCache)
 from .return_type import ReturnType
 
 __all__ = ['BertEmbeddings', 'BertIntermediate', 'BertOutput', 'BertAttention', 'BertLayer', 'BertEncoder', 'BertModel',
@@ -16,4 +18,5 @@ __all__ = ['BertEmbeddings', 'BertIntermediate', 'BertOutput', 'BertAttention', 
            'PositionwiseFeedForward', 'QBertIntermediate', 'QBertOutput', 'QBertLayer', 'QBertEncoder', 'QBertModel', 'GPT2Model',
            'MultiHeadedAttentionSmartBatch', 'BertLayerSmartBatch', 'BertEncoderSmartBatch', 'BertModelSmartBatch',
            'BertModelNoPoolerSmartBatch', 'DistillBertAttention', 'DistrillFFN', 'DistrillTransformerBlock', 'DistrillTransformer',
-           'DistilBertModel', 'RobertaModel', 'AlbertAttention', 'AlbertLayer', 'AlbertLayerGroup', 'AlbertTransformer', 'AlbertModel', 'TransformerDecoderLayer', 'TransformerDecoder']
+           'DistilBertModel', 'RobertaModel', 'AlbertAttention', 'AlbertLayer', 'AlbertLayerGroup', 'AlbertTransformer', 'AlbertModel', 'TransformerDecoderLayer', 'TransformerDecoder',
+           'rotary', 'paged_append', 'paged_attention', 'paged_reserve', 'paged_fork', 'paged_copy', 'paged_compact', 'RotaryEmbedding', 'PagedKVCache']

@@ -1,0 +1,330 @@
+"""Serving over a pool of cache pages: every sequence of a batch has its own length, its keys and values lie in pages anywhere in a pool, beams share what they
+have in common, and new tokens come one, a few, or a chunk of a prompt at a time.
+
+The functions are the operators themselves, on torch tensors; `PagedKVCache` holds the tensors that they work on, for a stack of layers, and `RotaryEmbedding` the
+frequencies of rotary positions. One step of a batch whose sequence b has new[b] new tokens, packed one sequence behind the other as rows of q, k, v:
+
+    cache = PagedKVCache(layers=24, pages=20000, sequences=64, max_tokens=4096, kv_heads=8, head_size=128)
+    rotary = RotaryEmbedding(128, device="cuda")
+    granted = cache.reserve(new)                           # pages for the new tokens (int32 [64] on the device)
+    for layer in ...:
+        q = cache.append(layer, k, v, cu_seqlens, q=q, rotary=rotary)
+        context = cache.attend(layer, q, cu_seqlens)       # [tokens, heads, head_size]
+    cache.advance(new)
+    cache.fork(parents)                                    # beams follow their parents; -1 frees a row
+
+Nothing here waits for the device or reads from it, so that a step can be captured into a graph; what an index outside its table comes to is said in
+include/ttb.h, and device_status reports it. The reference has no counterpart: its decoder concatenates one cache of equally long sequences a step
+(multi_headed_attention.cpp:207-231).
+"""
+import math
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from .._cxx import cxx
+
+__all__ = ['rotary', 'paged_append', 'paged_attention', 'paged_reserve', 'paged_fork', 'paged_copy', 'paged_compact', 'RotaryEmbedding', 'PagedKVCache']
+
+_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _fail(name, why):
+    raise ValueError(f"{name} {why}")
+
+
+def _rows(t, name, d=None):
+    """(rows, heads, head size, elements between rows) of a [tokens, heads, d] tensor whose heads lie side by side."""
+    if t.dim() != 3:
+        _fail(name, "must be [tokens, heads, head size]")
+    (n, heads, width), (row, head, one) = t.shape, t.stride()
+    if width and (one != 1 and width > 1 or head != width and heads > 1):
+        _fail(name, "must have its heads side by side (strides [any, head size, 1])")
+    if d is not None and width != d:
+        _fail(name, f"must have heads of {d}")
+    return n, heads, width, row if n > 1 else heads * width
+
+
+def _same(device, **tensors):
+    for name, t in tensors.items():
+        if t.device != device:
+            _fail(name, f"is on {t.device}, not on {device}")
+
+
+def _index(t, name, shape, device, dtype=torch.int32):
+    if t.dtype != dtype or not t.is_contiguous() or t.device != device or tuple(t.shape) != shape:
+        _fail(name, f"must be a contiguous {dtype} tensor of {list(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _gpu(t, name):
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is not on a CUDA device: this runtime has no CPU path")
+    return t.device.index
+
+
+def _freqs(freqs, device):
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or freqs.device != device:
+        _fail("freqs", f"must be a contiguous float64 vector on {device}")
+    return freqs.data_ptr(), 2 * freqs.numel()
+
+
+def _kv(keys, values, table, cu_seqlens, past_lens, dtype, device):
+    """The arguments that describe one layer's pages."""
+    if keys.dim() != 4 or keys.shape != values.shape:
+        _fail("keys and values", "must be [pages, key heads, page tokens, head size], alike")
+    if keys.dtype != dtype or values.dtype != dtype:
+        _fail("keys and values", f"must be {dtype}, as the rows are")
+    _same(device, keys=keys, values=values, table=table)
+    pages, heads, tokens, d = keys.shape
+    strides = keys.stride()
+    if strides != values.stride() or strides[1:] != (tokens * d, d, 1):
+        _fail("keys and values", "must have contiguous pages, equally far apart")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 and table.shape[1] > 1:
+        _fail("table", "must be int32 [sequences, pages] with contiguous rows")
+    B, width = table.shape
+    cu, past = _index(cu_seqlens, "cu_seqlens", (B + 1,), device), _index(past_lens, "past_lens", (B,), device)
+    return (keys.data_ptr(), values.data_ptr(), strides[0] if pages > 1 else heads * tokens * d, pages, heads, tokens, d, table.data_ptr(),
+            table.stride(0) if B > 1 else width, width, cu, past, B)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
+           out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None):
+    """Rotary positions of q [tokens, heads, d] and k [tokens, key heads, d] (or None): returns (q, k) turned, in new tensors or in `out` (which may be (q, k)
+    themselves). positions: int64 [tokens]. freqs: float64 [n], radians a position; the first 2n elements of every head are turned, in pairs (i, i + n), or (2i, 2i + 1) if
+    interleaved, and their length is multiplied by scale."""
+    device = _gpu(q, "q")
+    if q.dtype not in _CODE:
+        _fail("q", "must be fp32, fp16 or bf16")
+    T, heads, d, ldq = _rows(q, "q")
+    at, turned = _freqs(freqs, q.device)
+    where = _index(positions, "positions", (T,), q.device, torch.int64)
+    kv_heads = ldk = 0
+    if k is not None:
+        n, kv_heads, _, ldk = _rows(k, "k", d)
+        if n != T or k.dtype != q.dtype:
+            _fail("k", "must have q's tokens and dtype")
+        _same(q.device, k=k)
+    if out is None:
+        q_out, k_out = torch.empty((T, heads, d), dtype=q.dtype, device=q.device), None if k is None else torch.empty((T, kv_heads, d), dtype=q.dtype, device=q.device)
+        ldq_out, ldk_out = heads * d, kv_heads * d
+    else:
+        q_out, k_out = out
+        for o, x, name in ((q_out, q, "out[0]"), (k_out, k, "out[1]")):
+            if (o is None) != (x is None) or o is not None and (o.shape != x.shape or o.dtype != x.dtype or o.device != x.device):
+                _fail(name, "must be like its input")
+        ldq_out, ldk_out = _rows(q_out, "out[0]")[3], 0 if k is None else _rows(k_out, "out[1]")[3]
+    cxx.rotary(device, _stream(device), _CODE[q.dtype], q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
+               ldq, ldk, ldq_out, ldk_out, T, heads, kv_heads, d, turned, where, at, interleaved, scale)
+    return q_out, k_out
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor,
+                 past_lens: torch.Tensor, *, q: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None, interleaved: bool = False, scale: float = 1.0,
+                 out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Files k and v [tokens, key heads, d] of new tokens as tokens past_lens[b] and following of their sequences. Sequence b's are rows cu_seqlens[b] to
+    cu_seqlens[b + 1]; table int32 [sequences, width] lists the pages of each; keys and values are the layer's pool [pages, key heads, page tokens, d]. With `freqs` (see
+    rotary) the keys are turned by their places on the way, and so is q, which is returned in a new tensor or in `out`."""
+    device = _gpu(k, "k")
+    if k.dtype not in _CODE:
+        _fail("k", "must be fp16 or bf16")
+    T, heads, d, ldk = _rows(k, "k")
+    n, other, _, ldv = _rows(v, "v", d)
+    if n != T or other != heads or v.dtype != k.dtype:
+        _fail("v", "must be like k")
+    kv = _kv(keys, values, table, cu_seqlens, past_lens, k.dtype, k.device)
+    if kv[4] != heads or kv[6] != d:
+        _fail("k", "must have the pool's heads")
+    _same(k.device, v=v)
+    if freqs is None:
+        if q is not None:
+            _fail("q", "is turned by freqs: it has none without them")
+        cxx.paged_append(device, _stream(device), _CODE[k.dtype], *kv, T, k.data_ptr(), ldk, v.data_ptr(), ldv, 0, 0, False, 1.0, 0, 0, 0, 0, 0)
+        return None
+    at, turned = _freqs(freqs, k.device)
+    qp = op = ldq = ldq_out = q_heads = 0
+    if q is not None:
+        n, q_heads, _, ldq = _rows(q, "q", d)
+        if n != T or q.dtype != k.dtype:
+            _fail("q", "must have k's tokens and dtype")
+        _same(k.device, q=q)
+        if out is None:
+            out = torch.empty((T, q_heads, d), dtype=q.dtype, device=q.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            _fail("out", "must be like q")
+        qp, op, ldq_out = q.data_ptr(), out.data_ptr(), _rows(out, "out")[3]
+    cxx.paged_append(device, _stream(device), _CODE[k.dtype], *kv, T, k.data_ptr(), ldk, v.data_ptr(), ldv, at, turned, interleaved, scale, qp, op, ldq, ldq_out,
+                     q_heads)
+    return out if q is not None else None
+
+
+def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor, past_lens: torch.Tensor, *,
+                    causal: bool = True, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [tokens, heads, d] over the pages of its sequences (arguments as for paged_append, whose new tokens have been filed): token i of a sequence sees its
+    cached tokens up to itself, or all past + new of them if not causal. heads is a multiple of the key heads; scale is d ** -0.5 unless given. Rows that belong to no sequence
+    are left as they are in `out`, undefined without it."""
+    device = _gpu(q, "q")
+    if q.dtype not in _CODE:
+        _fail("q", "must be fp16 or bf16")
+    T, heads, d, ldq = _rows(q, "q")
+    kv = _kv(keys, values, table, cu_seqlens, past_lens, q.dtype, q.device)
+    if kv[6] != d or heads % max(kv[4], 1):
+        _fail("q", "must have the pool's head size, and a multiple of its heads")
+    if out is None:
+        out = torch.empty((T, heads, d), dtype=q.dtype, device=q.device)
+        ldo = heads * d
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+            _fail("out", "must be like q")
+        ldo = _rows(out, "out")[3]
+    cxx.paged_attention(device, _stream(device), _CODE[q.dtype], *kv, q.data_ptr(), ldq, T, heads, causal, d ** -0.5 if scale is None else scale, out.data_ptr(), ldo)
+    return out
+
+
+def _tables(table, lens, refs):
+    device = _gpu(table, "table")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 and table.shape[1] > 1:
+        _fail("table", "must be int32 [sequences, pages] with contiguous rows")
+    B, width = table.shape
+    if refs.dim() != 1:
+        _fail("refs", "must be a vector")
+    return device, (table.data_ptr(), table.stride(0) if B > 1 else width, B, width, 0 if lens is None else _index(lens, "lens", (B,), table.device),
+                    _index(refs, "refs", tuple(refs.shape), table.device), refs.numel())
+
+
+def _pool(pool):
+    if pool.dim() < 3:
+        _fail("pool", "must be [planes, pages, ...]")
+    if not pool[0, 0].is_contiguous():
+        _fail("pool", "must have contiguous pages")
+    size, (planes, pages) = pool.element_size(), pool.shape[:2]
+    page = size * math.prod(pool.shape[2:])
+    page_stride = pool.stride(1) * size if pages > 1 else page
+    return pool.data_ptr(), planes, pool.stride(0) * size if planes > 1 else pages * page_stride, pages, page_stride, page
+
+
+def paged_reserve(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, new_tokens: torch.Tensor, page_tokens: int):
+    """Room for new_tokens[b] more tokens of every row of the page table: takes the lowest free pages (those of refs 0) into the table. A row that would write to a
+    page that other rows list too gets one of its own in its place. Returns (granted int32 [sequences], copies int32 [sequences, 2]); hand the copies to paged_copy before the new
+    tokens are filed. A row that is not granted (0) has been left alone: the pool is full, or its row of the table."""
+    device, t = _tables(table, lens, refs)
+    new = _index(new_tokens, "new_tokens", (t[2],), table.device)
+    granted, copies = torch.empty(t[2], dtype=torch.int32, device=table.device), torch.empty((t[2], 2), dtype=torch.int32, device=table.device)
+    cxx.paged_reserve(device, _stream(device), *t, new, page_tokens, granted.data_ptr(), copies.data_ptr())
+    return granted, copies
+
+
+def paged_fork(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor) -> None:
+    """Row b of the page table becomes what row parents[b] was, and shares its pages; parents[b] = -1 frees the row. table, lens and refs are changed in place."""
+    device, t = _tables(table, lens, refs)
+    cxx.paged_fork(device, _stream(device), *t, _index(parents, "parents", (t[2],), table.device))
+
+
+def paged_copy(pool: torch.Tensor, pairs: torch.Tensor) -> None:
+    """Page pairs[i, 1] of every plane of pool [planes, pages, ...] becomes a copy of page pairs[i, 0] (int32 [n, 2]; pairs with a negative entry are left out). A page that
+    is written may not be in another pair."""
+    device = _gpu(pool, "pool")
+    if pairs.dim() != 2:
+        _fail("pairs", "must be [n, 2]")
+    cxx.paged_copy(device, _stream(device), *_pool(pool), _index(pairs, "pairs", (pairs.shape[0], 2), pool.device), pairs.shape[0])
+
+
+def paged_compact(table: torch.Tensor, refs: torch.Tensor, pool: torch.Tensor) -> torch.Tensor:
+    """Moves the pages in use to the front of the pool, table and refs with them. Returns how many there are (int32 [1] on the device)."""
+    device, t = _tables(table, None, refs)
+    _same(table.device, pool=pool)
+    used = torch.empty(1, dtype=torch.int32, device=table.device)
+    cxx.paged_compact(device, _stream(device), *t, *_pool(pool), used.data_ptr())
+    return used
+
+
+class RotaryEmbedding:
+    """Frequencies of rotary positions, base ** (-2i / dim) radians a position for the pairs of the first `dim` elements of a head, and how they are stretched for contexts
+    `factor` times as long as the model was trained for:
+        None      as they are
+        "linear"  all divided by factor (positions are interpolated)
+        "ntk"     the base raised, so that the slowest is divided by factor and the fastest stays
+        "yarn"    those that turn more than `fast` times in `trained` tokens stay, those that turn less than `slow` times are divided by factor, a ramp over the pairs
+                  between; turned elements are scaled by 0.1 ln(factor) + 1
+    """
+
+    def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, stretch: Optional[str] = None, factor: float = 1.0, trained: int = 2048,
+                 fast: float = 32.0, slow: float = 1.0, device: Union[str, torch.device] = "cuda"):
+        if dim <= 0 or dim % 2:
+            raise ValueError("dim must be even and positive")
+        if stretch not in (None, "linear", "ntk", "yarn"):
+            raise ValueError(f"unknown stretch {stretch!r}")
+        if factor < 1.0 and stretch is not None:
+            raise ValueError("factor must be at least 1")
+        if stretch == "ntk":
+            base = base * factor ** (dim / max(dim - 2, 1))
+        freqs = base ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+        self.interleaved, self.scale = interleaved, 1.0
+        if stretch == "linear":
+            freqs = freqs / factor
+        elif stretch == "yarn":
+            # the pair (as a real number) that turns `turns` times in the trained length
+            pair = lambda turns: dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+            low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), dim - 1)
+            ramp = ((torch.arange(dim // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+            freqs = freqs / factor * ramp + freqs * (1 - ramp)
+            self.scale = 0.1 * math.log(factor) + 1.0
+        self.freqs = freqs.to(device)
+
+    def __call__(self, q, k, positions, out=None):
+        """rotary() of q and k at these positions."""
+        return rotary(q, k, positions, self.freqs, interleaved=self.interleaved, scale=self.scale, out=out)
+
+
+class PagedKVCache:
+    """The keys and values of a stack of layers in one pool of pages, and the sequences that they belong to. Row b of the page table is sequence b: `sequences` of them at once,
+    a row without tokens being free. `lens` (int32, on the device) are the tokens cached; advance() moves them on when all layers have filed a step's tokens."""
+
+    def __init__(self, layers: int, pages: int, sequences: int, max_tokens: int, kv_heads: int, head_size: int, page_tokens: int = 16,
+                 dtype: torch.dtype = torch.float16, device: Union[str, torch.device] = "cuda"):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise NotImplementedError("caches are provided for fp16 / bf16 models")
+        width = -(-max_tokens // page_tokens)
+        self.page_tokens = page_tokens
+        self.pool = torch.empty((2 * layers, pages, kv_heads, page_tokens, head_size), dtype=dtype, device=device)
+        self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(sequences, dtype=torch.int32, device=device)
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+
+    def _counts(self, values) -> torch.Tensor:
+        return values if isinstance(values, torch.Tensor) else torch.tensor(values, dtype=torch.int32).to(self.table.device)
+
+    def reserve(self, new_tokens: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
+        """Pages for new_tokens[b] more tokens of every sequence; pages that are shared and about to be written are copied. Returns what paged_reserve grants."""
+        granted, copies = paged_reserve(self.table, self.lens, self.refs, self._counts(new_tokens), self.page_tokens)
+        paged_copy(self.pool, copies)
+        return granted
+
+    def append(self, layer: int, k, v, cu_seqlens, q=None, rotary: Optional[RotaryEmbedding] = None, out=None):
+        """paged_append into a layer's pages; with `rotary`, q is returned turned."""
+        turn = {} if rotary is None else {"q": q, "freqs": rotary.freqs, "interleaved": rotary.interleaved, "scale": rotary.scale, "out": out}
+        if rotary is None and q is not None:
+            raise ValueError("q is turned by rotary positions: it has none without them")
+        return paged_append(k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.table, cu_seqlens, self.lens, **turn)
+
+    def attend(self, layer: int, q, cu_seqlens, causal: bool = True, scale: Optional[float] = None, out=None):
+        """paged_attention over a layer's pages, between append and advance."""
+        return paged_attention(q, self.pool[2 * layer], self.pool[2 * layer + 1], self.table, cu_seqlens, self.lens, causal=causal, scale=scale, out=out)
+
+    def advance(self, new_tokens: Union[torch.Tensor, Sequence[int]]) -> None:
+        """The new tokens are cached now."""
+        self.lens += self._counts(new_tokens)
+
+    def fork(self, parents: Union[torch.Tensor, Sequence[int]]) -> None:
+        """paged_fork: sequence b becomes what parents[b] was; -1 frees it."""
+        paged_fork(self.table, self.lens, self.refs, self._counts(parents))
+
+    def release(self, sequences: Sequence[int]) -> None:
+        """Frees these sequences' pages (those that no other lists)."""
+        gone = set(sequences)
+        self.fork([-1 if b in gone else b for b in range(self.table.shape[0])])
+
+    def compact(self) -> torch.Tensor:
+        """paged_compact: the pages in use move to the front of the pool."""
+        return paged_compact(self.table, self.refs, self.pool)
