@@ -8,10 +8,11 @@
 // the own loads until the tile's end, where the four states are joined, and the rings run on into the next tile meanwhile. Parts of a tile that
 // was cut go to a workspace in fp32 and a second kernel joins them, in the order of the keys.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
-#include "ttb_paged.cuh"
+#include "ttb_paged_attention.cuh"
 #include "ttb_sm100.cuh"
 
 using namespace ttb;
@@ -20,45 +21,11 @@ using namespace ttb::sm100;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kRows = 16;    // of a tile
-constexpr int kBlock = 32;   // keys of a warp's step
-constexpr int kUnit = kBlock * kWarps;
+constexpr int kRows = kFewRows;
+constexpr int kBlock = 32;  // keys of a warp's step
+static_assert(kBlock * kWarps == kUnit, "a step of the four warps is a unit");
 
-struct Params {
-  Sequences s;
-  Split split;
-  const void* q;
-  void* out;
-  long long ldq, ldo;
-  int group;        // query heads of a key head
-  float scale;      // times log2 e
-  float* part_o;    // [2 * CTAs][rows][d]: a CTA's first and last part
-  float2* part_ml;  // [2 * CTAs][rows]: maximum (log2 units) and sum
-  struct Cut* cuts; // [CTAs]
-};
-
-// A tile that was cut, written by the CTA that has its beginning.
-struct Cut {
-  int pieces;             // 0: none; the first is in slot `slot`, the others are the next CTAs' first parts
-  int slot, tok0, head0, rows, block_heads;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&h);
-}
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
@@ -75,103 +42,6 @@ template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// The places of the sequences in the line: prefix[b] units before sequence b; prefix[B] is returned. All threads of the block.
-__device__ __forceinline__ long long line_up(const Params& p, long long* prefix, long long* scratch, int threads) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  bool any_bad = false;
-  for (int b = tid; b < p.s.B; b += threads) {
-    bool bad;
-    const Sequence q = sequence_of(p.s, b, &bad);
-    any_bad |= bad;
-    prefix[b] = units_of_sequence(p.split, q.past, q.n);
-  }
-  if (any_bad && blockIdx.x == 0) bad_index(p.s.status);
-  __syncthreads();
-  long long carry = 0;
-  for (int b0 = 0; b0 < p.s.B; b0 += threads) {
-    const int b = b0 + tid;
-    const long long mine = b < p.s.B ? prefix[b] : 0;
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) scratch[warp] = incl;
-    __syncthreads();
-    long long before = carry;
-    for (int w = 0; w < threads / 32; ++w) {
-      if (w < warp) before += scratch[w];
-      carry += scratch[w];
-    }
-    if (b < p.s.B) prefix[b] = before + incl - mine;
-    __syncthreads();
-  }
-  if (tid == 0) prefix[p.s.B] = carry;
-  __syncthreads();
-  return carry;
-}
-
-// A stretch's next part: units [first, first + take) of one tile and head block.
-struct Part {
-  int b, block, take;
-  int tok0, rows, keys;   // first token's row of q, rows of the tile, keys of the sequence that the tile's last token sees
-  int pos0;               // the first token's place in the sequence
-  long long tile, units, first;
-  Sequence q;
-};
-
-__device__ __forceinline__ void fill_part(const Params& p, Part& t, long long left) {
-  const int tile0 = (int)t.tile * p.split.tile_tokens, n = min(p.split.tile_tokens, t.q.n - tile0);
-  t.tok0 = t.q.tok0 + tile0;
-  t.rows = n * p.split.block_heads;
-  t.pos0 = t.q.past + tile0;
-  t.keys = (int)min((long long)t.q.past + (p.split.causal ? tile0 + n : t.q.n), (long long)p.s.cap);
-  t.take = (int)min(left, t.units - t.first);
-}
-
-// The part at unit u, of which `left` are the stretch's.
-__device__ __forceinline__ Part part_at(const Params& p, const long long* prefix, long long u, long long left) {
-  int lo = 0, hi = p.s.B;  // the last sequence with prefix <= u (that of an empty sequence equals its successor's)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= u) lo = mid;
-    else hi = mid;
-  }
-  bool bad;
-  Part t;
-  t.b = lo;
-  t.q = sequence_of(p.s, lo, &bad);
-  const Place at = place_of(p.split, t.q.past, t.q.n, u - prefix[lo]);
-  t.tile = at.tile;
-  t.block = at.block;
-  t.units = at.units;
-  t.first = at.first;
-  fill_part(p, t, left);
-  return t;
-}
-
-// The part behind t, `left` units being left of the stretch (more than none).
-__device__ __forceinline__ void next_part(const Params& p, Part& t, long long left) {
-  t.first = 0;
-  if (++t.block == p.split.blocks) {
-    t.block = 0;
-    ++t.tile;
-    while (t.tile * p.split.tile_tokens >= t.q.n) {  // the next sequence that has new tokens: there is one
-      bool bad;
-      t.q = sequence_of(p.s, ++t.b, &bad);
-      t.tile = 0;
-    }
-    t.units = units_of_tile(p.split, t.q.past, t.q.n, t.tile);
-  }
-  fill_part(p, t, left);
-}
-
-// first query head of a head block, and how many of its rows per token exist (the last block of a key head may be short)
-__device__ __forceinline__ int first_head(const Params& p, int block) {
-  return block / p.split.head_blocks * p.group + block % p.split.head_blocks * p.split.block_heads;
 }
 
 template <int D> struct Shape {
@@ -215,7 +85,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   const long long total = line_up(p, prefix, reinterpret_cast<long long*>(smem + S::kScratch), kThreads);
   const int ctas = ctas_of(total, (int)gridDim.x, 1), cta = blockIdx.x;
   if (cta >= ctas) {
-    if (tid == 0) p.cuts[cta].pieces = 0;
+    if (tid == 0) p.parts.cuts[cta].pieces = 0;
     return;
   }
   const long long lo = first_unit(total, ctas, cta), hi = first_unit(total, ctas, cta + 1);
@@ -268,7 +138,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   bool ok = true;
   for (long long u = lo; u < hi;) {
     const int head0 = first_head(p, t.block);
-    const int heads = min(p.split.block_heads, p.group - t.block % p.split.head_blocks * p.split.block_heads);
+    const int heads = heads_of(p, t.block);
     // queries: rows lane / 4 and lane / 4 + 8, columns of mma fragments
     uint32_t qf[D / 16][4];
     int limit[2];  // keys that the row sees
@@ -425,30 +295,26 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         const int row = (lane >> 2) + r * 8, i = row / p.split.block_heads, g = row % p.split.block_heads;
         if (row >= t.rows || g >= heads) continue;
         if (whole) {
-          const float inv = L[r] > 0.f ? 1.f / L[r] : 0.f;
+          const float inv = L[r] == 0.f ? 0.f : 1.f / L[r];
           T* dst = static_cast<T*>(p.out) + (long long)(t.tok0 + i) * p.ldo + (long long)(head0 + g) * D + (lane & 3) * 2;
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) *reinterpret_cast<uint32_t*>(dst + n * 8) = pack2<T>(o[n][2 * r] * inv, o[n][2 * r + 1] * inv);
         } else {
-          float* dst = p.part_o + ((long long)slot * kRows + row) * D + (lane & 3) * 2;
+          float* dst = p.parts.o + ((long long)slot * kRows + row) * D + (lane & 3) * 2;
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
-          if ((lane & 3) == 0) p.part_ml[(long long)slot * kRows + row] = make_float2(M[r], L[r]);
+          if ((lane & 3) == 0) p.parts.ml[(long long)slot * kRows + row] = make_float2(M[r], L[r]);
         }
       }
     }
     if (!whole && t.first == 0) {  // the tile's beginning is here, its rest the next CTAs'
       cut_here = true;
-      if (tid == 0) {
-        int pieces = 1;
-        while (cta + pieces < ctas && first_unit(total, ctas, cta + pieces) < u + t.units) ++pieces;
-        p.cuts[cta] = Cut{pieces, slot, t.tok0, head0, t.rows, heads};
-      }
+      if (tid == 0) p.parts.cuts[cta] = cut_of(p, t, u, total, cta, ctas, slot);
     }
     u += t.take;
     if (u < hi) next_part(p, t, hi - u);
   }
-  if (!cut_here && tid == 0) p.cuts[cta].pieces = 0;
+  if (!cut_here && tid == 0) p.parts.cuts[cta].pieces = 0;
   __syncthreads();
   if (*abort_flag) {
     if (tid == 0) atomicExch(p.s.status, (int)TTB_ERR_DEVICE_WAIT);
@@ -458,22 +324,31 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   }
 }
 
-// Joins the parts of the tiles that were cut: a block for each CTA of the kernel before, a warp for each row, parts in the order of the keys.
+// Joins the parts of the tiles that were cut, of both kernels: a block (and its neighbours along y) for each of their CTAs, a warp for each row, parts in the
+// order of the keys.
+struct JoinParams {
+  Parts parts[2];
+  int rows[2];
+  void* out;
+  long long ldo;
+};
 template <typename T, int D>
 __global__ void __launch_bounds__(128)
-paged_join_kernel(const Params p, int rows) {
+paged_join_kernel(const JoinParams p) {
   pdl_trigger();
   pdl_wait();
-  const Cut c = p.cuts[blockIdx.x];
+  const int which = blockIdx.z, lane = threadIdx.x & 31;
+  const Parts parts = which ? p.parts[1] : p.parts[0];
+  const int stride = which ? p.rows[1] : p.rows[0];
+  const Cut c = parts.cuts[blockIdx.x];
   if (c.pieces == 0) return;
-  const int lane = threadIdx.x & 31;
   constexpr int V = D / 32;
   for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < c.rows; row += gridDim.y * 4) {
-    const int i = row / p.split.block_heads, g = row % p.split.block_heads;
-    if (g >= c.block_heads) continue;
-    auto slot = [&](int k) { return (long long)(k == 0 ? c.slot : 2 * ((int)blockIdx.x + k)) * rows + row; };
+    const int i = row / c.block_heads, g = row % c.block_heads;
+    if (g >= c.heads) continue;
+    auto at = [&](int k) { return (long long)(k == 0 ? c.slot : 2 * ((int)blockIdx.x + k)) * stride + row; };
     float M = -INFINITY;
-    for (int k = lane; k < c.pieces; k += 32) M = fmaxf(M, p.part_ml[slot(k)].x);
+    for (int k = lane; k < c.pieces; k += 32) M = fmaxf(M, parts.ml[at(k)].x);
     M = warp_max(M);
     const float sub = M == -INFINITY ? 0.f : M;
     float L = 0.f, o[V];
@@ -481,13 +356,15 @@ paged_join_kernel(const Params p, int rows) {
     for (int v = 0; v < V; ++v) o[v] = 0.f;
 #pragma unroll 4
     for (int k = 0; k < c.pieces; ++k) {
-      const float2 ml = p.part_ml[slot(k)];
+      const float2 ml = parts.ml[at(k)];
       const float w = ex2(ml.x - sub);
       L = fmaf(ml.y, w, L);
+      if (w != 0.f) {  // a part without a key for this row has no sums
 #pragma unroll
-      for (int v = 0; v < V; ++v) o[v] = fmaf(p.part_o[slot(k) * D + v * 32 + lane], w, o[v]);
+        for (int v = 0; v < V; ++v) o[v] = fmaf(parts.o[at(k) * D + v * 32 + lane], w, o[v]);
+      }
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
     T* dst = static_cast<T*>(p.out) + (long long)(c.tok0 + i) * p.ldo + (long long)(c.head0 + g) * D;
 #pragma unroll
     for (int v = 0; v < V; ++v) dst[v * 32 + lane] = from_f<T>(o[v] * inv);
@@ -495,14 +372,13 @@ paged_join_kernel(const Params p, int rows) {
 }
 
 template <typename T, int D>
-int launch_rows(ttb_ctx* ctx, const ttb_paged_kv* kv, Params& p) {
+int launch_rows(ttb_ctx* ctx, const ttb_paged_kv* kv, const Params& p) {
   using S = Shape<D>;
   CUtensorMap tm_k, tm_v;
-  const bool bf16 = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value;
   const uint32_t box_rows = (uint32_t)std::min<int64_t>(kv->page_tokens, kBlock);
   for (int i = 0; i < 2; ++i)
-    if (!encode_tile_map_3d(i ? &tm_v : &tm_k, i ? kv->values : kv->keys, bf16, (uint64_t)kv->pages, (uint64_t)(kv->kv_heads * kv->page_tokens), D,
-                            (uint64_t)kv->page_stride, D, 1, box_rows))
+    if (!encode_tile_map_3d(i ? &tm_v : &tm_k, i ? kv->values : kv->keys, std::is_same<T, __nv_bfloat16>::value, (uint64_t)kv->pages,
+                            (uint64_t)(kv->kv_heads * kv->page_tokens), D, (uint64_t)kv->page_stride, D, 1, box_rows))
       return fail(ctx, TTB_ERR_CUDA, "paged_attention: the pools' tensor map was refused");
   static bool configured[64] = {};
   const int dev = ctx->device < 64 ? ctx->device : 63;
@@ -510,18 +386,52 @@ int launch_rows(ttb_ctx* ctx, const ttb_paged_kv* kv, Params& p) {
     TTB_CUDA(ctx, cudaFuncSetAttribute(paged_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     configured[dev] = true;
   }
+  launch_pdl(paged_rows_kernel<T, D>, dim3((unsigned)ctx->sm_count), dim3(kThreads), S::kBytes, ctx->stream, tm_k, tm_v, p);
+  return launched(ctx, "paged_attention");
+}
+
+template <typename T, int D>
+int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, Params& p) {
+  // Which kernel: sequences whose new tokens make kFewRows rows at most go to the one for few rows, the others to the other. The host knows the lengths'
+  // sum only: with no more tokens than sequences one kernel takes all, whatever a single sequence has.
+  const int few = p.group <= kFewRows ? kFewRows / p.group : 0;
+  const bool one = kv->B == 1, rows_only = few > 0 && p.s.tokens <= (one ? few : (int)kv->B), many_only = few == 0 || (one && !rows_only);
   const int ctas = ctx->sm_count;
+  size_t at = 0, o[2], ml[2], cuts[2];
+  const int rows[2] = {kFewRows, kManyRows};
+  const bool used[2] = {!many_only, !rows_only};
+  auto take = [&](size_t bytes) { const size_t x = at; at = (at + bytes + 255) & ~(size_t)255; return x; };
+  for (int i = 0; i < 2; ++i) {
+    if (!used[i]) continue;
+    o[i] = take((size_t)2 * ctas * rows[i] * D * 4);
+    ml[i] = take((size_t)2 * ctas * rows[i] * 8);
+    cuts[i] = take((size_t)ctas * sizeof(Cut));
+  }
   void* ws = nullptr;
-  const size_t o_bytes = (size_t)2 * ctas * kRows * D * 4, ml_bytes = (size_t)2 * ctas * kRows * 8;
-  int st = ttb_alloc(ctx, o_bytes + ml_bytes + (size_t)ctas * sizeof(Cut), "paged_attention/parts", &ws);
+  int st = ttb_alloc(ctx, at, "paged_attention/parts", &ws);
   if (st) return st;
-  p.part_o = static_cast<float*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + o_bytes);
-  p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(ws) + o_bytes + ml_bytes);
-  launch_pdl(paged_rows_kernel<T, D>, dim3((unsigned)ctas), dim3(kThreads), S::kBytes, ctx->stream, tm_k, tm_v, p);
-  st = launched(ctx, "paged_attention");
+  JoinParams j = {};
+  j.out = p.out;
+  j.ldo = p.ldo;
+  int n = 0;
+  for (int i = 0; i < 2 && !st; ++i) {
+    if (!used[i]) continue;
+    char* base = static_cast<char*>(ws);
+    p.parts = Parts{reinterpret_cast<float*>(base + o[i]), reinterpret_cast<float2*>(base + ml[i]), reinterpret_cast<Cut*>(base + cuts[i])};
+    p.low = i == 0 || many_only ? 0 : few + 1;
+    p.high = i == 1 || rows_only ? INT_MAX : few;
+    j.parts[n] = p.parts;
+    j.rows[n++] = rows[i];
+    if (i == 0) {
+      p.split = split_of((int)heads, (int)kv->kv_heads, kFewRows, 1, kUnit, p.split.causal);
+      st = launch_rows<T, D>(ctx, kv, p);
+    } else {
+      p.split = split_of((int)heads, (int)kv->kv_heads, kManyRows / 2, 2, kUnit, p.split.causal);
+      st = paged_tc_launch(ctx, dtype, kv, heads, p);
+    }
+  }
   if (!st) {
-    launch_pdl(paged_join_kernel<T, D>, dim3((unsigned)ctas, kRows / 4), dim3(128), 0, ctx->stream, p, kRows);
+    launch_pdl(paged_join_kernel<T, D>, dim3((unsigned)ctas, used[1] ? 16 : kFewRows / 4, (unsigned)n), dim3(128), 0, ctx->stream, j);
     st = launched(ctx, "paged_attention_join");
   }
   const int f = ttb_free(ctx, ws, "paged_attention/parts");
@@ -550,7 +460,7 @@ extern "C" int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* 
   p.ldo = ldo;
   p.group = (int)(heads / kv->kv_heads);
   p.scale = scale * kLog2e;
-  p.split = split_of((int)heads, (int)kv->kv_heads, kRows, 1, kUnit, causal != 0);
-  if (kv->d == 64) return dtype == TTB_F16 ? launch_rows<__half, 64>(ctx, kv, p) : launch_rows<__nv_bfloat16, 64>(ctx, kv, p);
-  return dtype == TTB_F16 ? launch_rows<__half, 128>(ctx, kv, p) : launch_rows<__nv_bfloat16, 128>(ctx, kv, p);
+  p.split.causal = causal != 0;
+  if (kv->d == 64) return dtype == TTB_F16 ? launch_all<__half, 64>(ctx, dtype, kv, heads, p) : launch_all<__nv_bfloat16, 64>(ctx, dtype, kv, heads, p);
+  return dtype == TTB_F16 ? launch_all<__half, 128>(ctx, dtype, kv, heads, p) : launch_all<__nv_bfloat16, 128>(ctx, dtype, kv, heads, p);
 }

@@ -1,0 +1,172 @@
+// What the two kernels of the attention over cache pages share: a call's parameters, the places of its tiles in the line of units (ttb_paged_rules.cuh), and the
+// parts of tiles that were cut.
+#pragma once
+#include "ttb_paged.cuh"
+
+namespace ttb {
+namespace paged {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnit = 128;    // keys
+constexpr int kFewRows = 16;  // of a tile of the kernel for few rows
+constexpr int kManyRows = 256;
+
+// A tile that was cut, written by the CTA that has its beginning.
+struct Cut {
+  int pieces;  // 0: none; the first is in slot `slot`, the others are the next CTAs' first parts
+  int slot, tok0, head0, rows, block_heads, heads;  // rows: token * block_heads + head, of which the first `heads` exist
+};
+
+struct Parts {
+  float* o;    // [2 * CTAs][rows of a tile][d]: a CTA's first and last part, sums of values
+  float2* ml;  // [2 * CTAs][rows of a tile]: maximum (log2 units) and sum
+  Cut* cuts;   // [CTAs]
+};
+
+struct Params {
+  Sequences s;
+  Split split;
+  const void* q;
+  void* out;
+  long long ldq, ldo;
+  int group;      // query heads of a key head
+  int low, high;  // the kernel takes the sequences of low to high new tokens
+  float scale;    // times log2 e
+  Parts parts;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+// Sequence b, without new tokens where it is the other kernel's.
+__device__ __forceinline__ Sequence taken(const Params& p, int b, bool* bad) {
+  Sequence q = sequence_of(p.s, b, bad);
+  if (q.n < p.low || q.n > p.high) q.n = 0;
+  return q;
+}
+
+// The places of the sequences in the line: prefix[b] units before sequence b; prefix[B] is returned. All threads of the block.
+__device__ __forceinline__ long long line_up(const Params& p, long long* prefix, long long* scratch, int threads) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  bool any_bad = false;
+  for (int b = tid; b < p.s.B; b += threads) {
+    bool bad;
+    const Sequence q = taken(p, b, &bad);
+    any_bad |= bad;
+    prefix[b] = units_of_sequence(p.split, q.past, q.n);
+  }
+  if (any_bad && blockIdx.x == 0) bad_index(p.s.status);
+  __syncthreads();
+  long long carry = 0;
+  for (int b0 = 0; b0 < p.s.B; b0 += threads) {
+    const int b = b0 + tid;
+    const long long mine = b < p.s.B ? prefix[b] : 0;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    long long before = carry;
+    for (int w = 0; w < threads / 32; ++w) {
+      if (w < warp) before += scratch[w];
+      carry += scratch[w];
+    }
+    if (b < p.s.B) prefix[b] = before + incl - mine;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[p.s.B] = carry;
+  __syncthreads();
+  return carry;
+}
+
+// A stretch's next part: units [first, first + take) of one tile and head block.
+struct Part {
+  int b, block, take;
+  int tok0, rows, keys;   // first token's row of q, rows of the tile, keys of the sequence that the tile's last token sees
+  int pos0;               // the first token's place in the sequence
+  long long tile, units, first;
+  Sequence q;
+};
+
+__device__ __forceinline__ void fill_part(const Params& p, Part& t, long long left) {
+  const int tile0 = (int)t.tile * p.split.tile_tokens, n = min(p.split.tile_tokens, t.q.n - tile0);
+  t.tok0 = t.q.tok0 + tile0;
+  t.rows = n * p.split.block_heads;
+  t.pos0 = t.q.past + tile0;
+  t.keys = (int)min((long long)t.q.past + (p.split.causal ? tile0 + n : t.q.n), (long long)p.s.cap);
+  t.take = (int)min(left, t.units - t.first);
+}
+
+// The part at unit u, of which `left` are the stretch's.
+__device__ __forceinline__ Part part_at(const Params& p, const long long* prefix, long long u, long long left) {
+  int lo = 0, hi = p.s.B;  // the last sequence with prefix <= u (that of an empty sequence equals its successor's)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  bool bad;
+  Part t;
+  t.b = lo;
+  t.q = taken(p, lo, &bad);
+  const Place at = place_of(p.split, t.q.past, t.q.n, u - prefix[lo]);
+  t.tile = at.tile;
+  t.block = at.block;
+  t.units = at.units;
+  t.first = at.first;
+  fill_part(p, t, left);
+  return t;
+}
+
+// The part behind t, `left` units being left of the stretch (more than none).
+__device__ __forceinline__ void next_part(const Params& p, Part& t, long long left) {
+  t.first = 0;
+  if (++t.block == p.split.blocks) {
+    t.block = 0;
+    ++t.tile;
+    while (t.tile * p.split.tile_tokens >= t.q.n) {  // the next sequence that has new tokens: there is one
+      bool bad;
+      t.q = taken(p, ++t.b, &bad);
+      t.tile = 0;
+    }
+    t.units = units_of_tile(p.split, t.q.past, t.q.n, t.tile);
+  }
+  fill_part(p, t, left);
+}
+
+// first query head of a head block, and how many of its rows per token exist (the last block of a key head may be short)
+__device__ __forceinline__ int first_head(const Params& p, int block) {
+  return block / p.split.head_blocks * p.group + block % p.split.head_blocks * p.split.block_heads;
+}
+
+// The query heads of a head block that exist (the last block of a key head may be short).
+__device__ __forceinline__ int heads_of(const Params& p, int block) {
+  return min(p.split.block_heads, p.group - block % p.split.head_blocks * p.split.block_heads);
+}
+
+// Whoever has the beginning of a tile that ends in another CTA's stretch, at unit u of the line, says so.
+__device__ __forceinline__ Cut cut_of(const Params& p, const Part& t, long long u, long long total, int cta, int ctas, int slot) {
+  int pieces = 1;
+  while (cta + pieces < ctas && first_unit(total, ctas, cta + pieces) < u + t.units) ++pieces;
+  return Cut{pieces, slot, t.tok0, first_head(p, t.block), t.rows, p.split.block_heads, heads_of(p, t.block)};
+}
+
+// The kernel for many rows (ttb_paged_attention_tc.cu) on tiles of kManyRows: launches it, parts of cut tiles going to p.parts.
+int paged_tc_launch(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, const Params& p);
+
+}  // namespace paged
+}  // namespace ttb
