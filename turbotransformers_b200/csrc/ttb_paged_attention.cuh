@@ -1,7 +1,10 @@
 // What the two kernels of the attention over cache pages share: a call's parameters, the places of its tiles in the line of units (ttb_paged_rules.cuh), and the
 // parts of tiles that were cut.
 #pragma once
+#include <algorithm>
+
 #include "ttb_paged.cuh"
+#include "ttb_sm100.cuh"
 
 namespace ttb {
 namespace paged {
@@ -55,6 +58,10 @@ __device__ __forceinline__ Sequence taken(const Params& p, int b, bool* bad) {
   if (q.n < p.low || q.n > p.high) q.n = 0;
   return q;
 }
+
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
 
 // The places of the sequences in the line: prefix[b] units before sequence b; prefix[B] is returned. All threads of the block.
 __device__ __forceinline__ long long line_up(const Params& p, long long* prefix, long long* scratch, int threads) {
@@ -161,8 +168,18 @@ __device__ __forceinline__ int heads_of(const Params& p, int block) {
 // Whoever has the beginning of a tile that ends in another CTA's stretch, at unit u of the line, says so.
 __device__ __forceinline__ Cut cut_of(const Params& p, const Part& t, long long u, long long total, int cta, int ctas, int slot) {
   int pieces = 1;
+#pragma unroll 1
   while (cta + pieces < ctas && first_unit(total, ctas, cta + pieces) < u + t.units) ++pieces;
   return Cut{pieces, slot, t.tok0, first_head(p, t.block), t.rows, p.split.block_heads, heads_of(p, t.block)};
+}
+
+// The tensor maps: boxes of `tokens` tokens of a head block's queries, of a page (128 tokens at most) of one key head's keys and values; 64 elements wide each.
+inline bool encode_maps(const ttb_paged_kv* kv, bool bf16, int64_t heads, const Params& p, int tokens, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
+  const uint32_t box_rows = (uint32_t)std::min<int64_t>(kv->page_tokens, kUnit);
+  const uint64_t pages = (uint64_t)kv->pages, rows = (uint64_t)(kv->kv_heads * kv->page_tokens), stride = (uint64_t)kv->page_stride, d = (uint64_t)kv->d;
+  return sm100::encode_tile_map_3d(q, p.q, bf16, (uint64_t)p.s.tokens, (uint64_t)heads, d, (uint64_t)p.ldq, d, (uint32_t)tokens, (uint32_t)p.split.block_heads) &&
+         sm100::encode_tile_map_3d(k, kv->keys, bf16, pages, rows, d, stride, d, 1, box_rows) &&
+         sm100::encode_tile_map_3d(v, kv->values, bf16, pages, rows, d, stride, d, 1, box_rows);
 }
 
 // The kernel for many rows (ttb_paged_attention_tc.cu) on tiles of kManyRows: launches it, parts of cut tiles going to p.parts.

@@ -4,12 +4,13 @@
 // One CTA an SM walks its stretch of the line (ttb_paged_rules.cuh). A tile is two sets of 128 query rows (tokens x heads of a key head) that share every key and value
 // tile of 128 tokens, so that 64 KB of them (heads of 128) feed 2 x 128 rows: with a set alone the tensor cores would want them twice as fast. A tile whose rows all
 // fit one set (a few tokens) puts them into both: the sets take the key tiles in turn and are joined at the tile's end, so that one's products still run beside the other's softmax.
-//   warp 0      : loads - a lane for each box (a page, or 128 keys) and half of a head: queries, then keys and values in turn through one ring
-//   warp 1      : matrix products - S = Q K^T (128 x 128, fp32 in TMEM), O += P V with P in TMEM over the scores it came from, V as it lies. Of a set the
-//                 order is QK(0), PV(0), QK(1), PV(1), ..., the other set's products between; everything a product waits for but the softmax is a barrier poll.
-//                 Rows of V behind the last key are set to zero here: a probability of zero would not undo what the page happens to hold.
-//   warps 4..11 : softmax, a warpgroup a set, a row a thread: scores from TMEM, exp2 with the scale folded in, P back to TMEM in 16 bits. The row's maximum is that of its
-//                 first tile; it is raised (and O rescaled) only where a tile's sum passes 2^15: the division by the sum makes the result independent of it.
+//   warps 0, 2  : loads - a lane for each box (a page, or 128 keys) and half of a head, half of them a warp's (a copy takes its thread some 60 cycles to issue,
+//                 one lane after the other): queries, and keys and values in turn through one ring
+//   warps 1, 3  : matrix products of a set each - S = Q K^T (128 x 128, fp32 in TMEM), O += P V with P in TMEM over the scores it came from, V as it lies, in
+//                 the order QK(0), PV(0), QK(1), PV(1), ...; everything a product waits for but the softmax is a barrier poll. Rows of V behind the last key are
+//                 set to zero here: a probability of zero would not undo what the page happens to hold.
+//   warps 4..11 : softmax, a warpgroup a set, a row a thread: scores from TMEM, exp2 with the scale folded in, P back to TMEM in 16 bits. The row's reference is the maximum of
+//                 its first tile; it is raised (and O rescaled) only where the sum of 32 probabilities passes 2^15: the division by the sum makes the result independent of it.
 // A tile's output is written while the next one's first scores are made. Every wait is bounded.
 #include <algorithm>
 #include <type_traits>
@@ -23,12 +24,27 @@ using namespace ttb::sm100;
 
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 384, kLoaders = 2;
 constexpr int kSet = kManyRows / 2;      // rows of a set
 constexpr int kHalf = kUnit * 128;       // bytes of 128 rows of 64 elements
 constexpr uint32_t kTmemCols = 512;
-constexpr float kRowSumLimit = 32768.0f;  // a tile row sum below this keeps every probability inside fp16 / bf16 range
+constexpr float kSumLimit = 32768.0f;  // a sum of probabilities below this keeps each of them inside fp16's and bf16's range
 static_assert(kUnit == 128 && kSet == 128, "the products are 128 x 128");
+
+// A part of the line as the CTA's warps read it: one of them works it out, the others would have its code in the instruction cache besides (with it in every role the kernel
+// was 192 KB long, and the products stood still for instructions).
+struct Work {
+  int units;       // that have keys; -1: there is no more
+  int turns;       // both sets hold the same rows and take the units in turn
+  int count[2];    // each set's units
+  int first;       // the part's first unit in its tile
+  int b, key_row;  // sequence, and the key head's first row in a page
+  int keys, pos0, tok0, rows;  // as in Part
+  int head0, heads;
+  int slot;        // of its sums, -1: the tile is whole
+  int pad[2];
+};
+constexpr int kRingWorks = 8;
 
 template <int D> struct Shape {
   static constexpr int kHalves = D / 64;
@@ -40,31 +56,59 @@ template <int D> struct Shape {
   static constexpr int kStats = kExchange + 4 * 16 * 32 * 4;        // float2 [4 warps][32 rows]
   static constexpr int kPrefix = kStats + 4 * 32 * 8;
   static constexpr int kScratch = kPrefix + (kMaxSequences + 1) * 8;
-  static constexpr int kBars = kScratch + kThreads / 32 * 8;
-  static constexpr int kNumBars = 10 + 2 * kStages + 8;
+  static constexpr int kWorks = kScratch + kThreads / 32 * 8;
+  static constexpr int kBars = kWorks + kRingWorks * (int)sizeof(Work);
+  static constexpr int kFirstSlotBar = 19 + 2 * kRingWorks;
+  static constexpr int kNumBars = kFirstSlotBar + 6 * kStages;
   static constexpr int kBytes = kBars + kNumBars * 8 + 16;
 };
 
-// How a part's units fall to the two sets.
-struct Sets {
-  bool turns;      // both hold the same rows and take the units in turn
-  int units;       // of the part that have keys
-  int count[2];    // each set's
-};
-__device__ __forceinline__ Sets sets_of(const Params& p, const Part& t) {
+// mbar_wait in few instructions, for the same reason as Work: a round lasts up to kSuspendHintNs, some 40 ns at least.
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (int i = 0; i < 1 << 18; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+
+// 2^x on the fp32 pipe, for one probability in eight, which the special-function unit is the limit of: 2^n * 2^f with n the nearest whole number, and 2^f on [-1/2, 1/2] by
+// a polynomial fitted to the least relative error (2^-18.5, far below P's rounding). A score that is no number or far above the reference gives 2^127, which the row sum tells.
+__device__ __forceinline__ float ex2_poly(float x) {
+  x = fmaxf(fminf(x, 127.f), -126.f);
+  const float n = x + 12582912.f;  // 3 * 2^22: the sum's last bit is one
+  const float f = x - (n - 12582912.f);
+  const float y = fmaf(fmaf(fmaf(fmaf(0.009570102207362652f, f, 0.05591786280274391f), f, 0.240247443318367f), f, 0.6931217908859253f), f, 0.9999992847442627f);
+  return __int_as_float(__float_as_int(y) + (__float_as_int(n) << 23));
+}
+
+__device__ __forceinline__ Work work_of(const Params& p, const Part& t, int slot) {
   const int tokens = p.split.tile_tokens / 2;  // of a set
-  Sets s;
-  s.turns = t.rows <= tokens * p.split.block_heads;
-  s.units = max(0, min(t.take, (t.keys + kUnit - 1) / kUnit - (int)t.first));
-  if (s.turns) {
-    s.count[0] = (s.units + 1) / 2;
-    s.count[1] = s.units / 2;
+  Work w;
+  w.turns = t.rows <= tokens * p.split.block_heads;
+  w.units = max(0, min(t.take, (t.keys + kUnit - 1) / kUnit - (int)t.first));
+  if (w.turns) {
+    w.count[0] = (w.units + 1) / 2;
+    w.count[1] = w.units / 2;
   } else {
     const int keys = p.split.causal ? min(t.pos0 + tokens, t.keys) : t.keys;
-    s.count[0] = max(0, min(s.units, (keys + kUnit - 1) / kUnit - (int)t.first));
-    s.count[1] = s.units;
+    w.count[0] = max(0, min(w.units, (keys + kUnit - 1) / kUnit - (int)t.first));
+    w.count[1] = w.units;
   }
-  return s;
+  w.first = (int)t.first;
+  w.b = t.b;
+  w.key_row = t.block / p.split.head_blocks << p.s.page_shift;
+  w.keys = t.keys;
+  w.pos0 = t.pos0;
+  w.tok0 = t.tok0;
+  w.rows = t.rows;
+  w.head0 = first_head(p, t.block);
+  w.heads = heads_of(p, t.block);
+  w.slot = t.take == t.units ? -1 : slot;
+  w.pad[0] = w.pad[1] = 0;
+  return w;
 }
 
 template <typename T, int D>
@@ -86,18 +130,31 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   auto o_done = [&](int s) { return bar(8 + s); };
   auto ex_full = [&](int quad) { return bar(10 + quad); };
   auto ex_empty = [&](int quad) { return bar(14 + quad); };
-  auto kv_full = [&](uint32_t g) { return bar(18 + (int)(g % S::kStages)); };
-  auto kv_empty = [&](uint32_t g) { return bar(18 + S::kStages + (int)(g % S::kStages)); };
+  auto q_empty_b = [&]() { return bar(18); };  // the first queries' buffer, by the second set where both read it
+  // A tile has landed for the first set, the second, or both (2). A wait tells a phase from the next and not from the one after: a barrier's waiters have to
+  // wait for its every phase, so that a tile that one set passes over is not told to it.
+  auto part_full = [&](uint32_t n) { return bar(19 + (int)(n % kRingWorks)); };
+  auto part_empty = [&](uint32_t n) { return bar(19 + kRingWorks + (int)(n % kRingWorks)); };
+  auto kv_full = [&](int f, uint32_t g) { return bar(S::kFirstSlotBar + f * S::kStages + (int)(g % S::kStages)); };
+  auto kv_empty = [&](int s, uint32_t g) { return bar(S::kFirstSlotBar + (3 + s) * S::kStages + (int)(g % S::kStages)); };  // by the sets that read the tile
+  auto v_zero = [&](uint32_t g) { return bar(S::kFirstSlotBar + 5 * S::kStages + (int)(g % S::kStages)); };
   auto kv_tile = [&](uint32_t g) { return base + S::kRing + (g % S::kStages) * S::kTile; };
-  auto kv_phase = [&](uint32_t g) { return (g / S::kStages) & 1u; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* passed = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [2]: units whose products a set has sent out, or passed over
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_trigger();
   if (threadIdx.x == 0) {
-    for (int k = 0; k < S::kNumBars; ++k) mbar_init(bar(k), k == 6 || k == 7 ? 4 : 1);  // p_ready: the set's four warps
+    for (int k = 0; k < S::kNumBars; ++k) {
+      int count = 1;
+      if (k == 6 || k == 7) count = 4;                                                            // p_ready: the set's four warps
+      if (k >= 19 + kRingWorks && k < 19 + 2 * kRingWorks) count = kThreads / 32 - 1;             // part_empty: all warps but the one that fills it
+      if (k >= S::kFirstSlotBar && k < S::kFirstSlotBar + 3 * S::kStages) count = kLoaders;       // kv_full
+      mbar_init(bar(k), count);
+    }
     *abort_flag = 0;
+    passed[0] = passed[1] = 0;
     mbar_init_fence();
   }
   if (warp == 1) tmem_alloc(smem_u32(tmem_slot), kTmemCols);
@@ -116,147 +173,221 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const long long lo = cta < ctas ? first_unit(total, ctas, cta) : 0, hi = cta < ctas ? first_unit(total, ctas, cta + 1) : 0;
   if (cta >= ctas && threadIdx.x == 0) p.parts.cuts[cta].pieces = 0;
   const int set_tokens = p.split.tile_tokens / 2;
+  Work* works = reinterpret_cast<Work*>(smem + S::kWorks);
+  // The n-th part, for every warp but the one that works them out. False: no part, there are no more or something gave up.
+  auto take_part = [&](uint32_t n, Work* w) {
+    const bool ok = __all_sync(0xffffffffu, wait_on(part_full(n), (n / kRingWorks) & 1u, abort_flag));
+    if (!ok) return false;
+    *w = works[n % kRingWorks];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(part_empty(n));
+    return w->units >= 0;
+  };
 
   if (cta < ctas && warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 0) {
+    if ((warp & 1) == 0) {
       // ------------------------------------------------------------------ loads
+      const int loader = warp >> 1;
       const int page_tokens = 1 << p.s.page_shift, box_rows = min(page_tokens, kUnit);
-      uint32_t g = 0, nq[2] = {0, 0};
-      bool ok = true;
-      Part t = part_at(p, prefix, lo, hi - lo);
-      for (long long u = lo; u < hi && ok;) {
-        const Sets sets = sets_of(p, t);
-        for (int i = 0; i < 2 * sets.units && ok; ++i) {
-          const int key0 = ((int)t.first + (i >> 1)) * kUnit;
-          const int boxes = (min(kUnit, t.keys - key0) + box_rows - 1) / box_rows;
-          const int box = lane / S::kHalves, half = lane % S::kHalves;
-          // a lane's page does not wait for the slot
-          int page = 0;
-          if (box < boxes) {
-            bool bad;
-            page = page_of(p.s, t.b, key0 + box * box_rows, &bad);
-            if (bad) {
+      const int at = lane * kLoaders + loader, box = at / S::kHalves, half = at % S::kHalves;
+      uint32_t g = 0, n_q = 0, n_b = 0, n = 0;
+      uint32_t used[2] = {0, 0}, parity[2] = {0, 0};  // a bit for each slot: whether the set reads what is there, and the phase of its kv_empty
+      bool ok = true, both = false;                   // both: the second set reads the first queries' buffer too
+      // The first loader works the parts out, one ahead of its own loads.
+      Part t;
+      long long u = lo;
+      bool cut_here = false;
+      auto publish = [&](Work* w) {
+        w->units = -1;
+        if (n > 0) u += t.take;
+        if (u < hi) {
+          if (n > 0) next_part(p, t, hi - u);
+          else t = part_at(p, prefix, lo, hi - lo);
+          *w = work_of(p, t, 2 * cta + (u == lo ? 0 : 1));
+          if (w->slot >= 0 && t.first == 0) {
+            cut_here = true;
+            if (lane == 0) p.parts.cuts[cta] = cut_of(p, t, u, total, cta, ctas, w->slot);
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok && wait_on(part_empty(n), ((n / kRingWorks) & 1u) ^ 1u, abort_flag));
+        if (ok && lane == 0) works[n % kRingWorks] = *w;
+        __syncwarp();
+        if (ok && lane == 0) mbar_arrive(part_full(n));
+        return ok && w->units >= 0;
+      };
+      // A lane's page is looked up a unit ahead (and looked at when it is needed), and serves its keys and values.
+      auto page_at = [&](const Work& w, int i) {
+        const int key = (w.first + i) * kUnit + box * box_rows;
+        return key < w.keys && box * box_rows < kUnit ? p.s.table[w.b * p.s.table_stride + (key >> p.s.page_shift)] : 0;
+      };
+      Work w = {}, w2;
+      int page = 0;
+      for (;; ++n) {  // w2 is the n-th part; the loads are those of w, the one before
+        const bool more = loader == 0 ? publish(&w2) : take_part(n, &w2);
+        if (w.units == 0 && more) page = page_at(w2, 0);  // at the beginning, and behind a part without keys (more tokens than the table lists)
+        for (int i = 0; i < w.units && ok; ++i) {
+          const int key = (w.first + i) * kUnit + box * box_rows, y = w.key_row + (key & (page_tokens - 1));
+          int mine = -1;
+          if (key < w.keys && box * box_rows < kUnit) {
+            mine = page;
+            if (mine < 0 || mine >= p.s.pages) {
               bad_index(p.s.status);
-              page = 0;
+              mine = 0;
             }
           }
-          ok = mbar_wait(kv_empty(g), kv_phase(g) ^ 1u, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          if (lane == 0) mbar_expect_tx(kv_full(g), (uint32_t)(boxes * box_rows * D * 2));
-          __syncwarp();
-          if (box < boxes) {
-            const int y = (t.block / p.split.head_blocks << p.s.page_shift) + ((key0 + box * box_rows) & (page_tokens - 1));
-            tma_load_3d(kv_tile(g) + half * kHalf + box * box_rows * 128, (i & 1) ? &tm_v : &tm_k, kv_full(g), half * 64, y, page);
-          }
-          ++g;
-          if (i == 0) {  // behind the first keys, which need no other tile to end
+          page = i + 1 < w.units ? page_at(w, i + 1) : more ? page_at(w2, 0) : 0;
+          const uint32_t bytes = (uint32_t)(__popc(__ballot_sync(0xffffffffu, mine >= 0)) * box_rows * 128);
+          const bool reads[2] = {w.turns ? (i & 1) == 0 : i < w.count[0], w.turns ? (i & 1) == 1 : true};
+#pragma unroll 1
+          for (int which = 0; which < 2; ++which, ++g) {  // keys, values
+            const uint32_t slot = 1u << (g % S::kStages);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-              if (!ok || sets.count[s] == 0 || (s == 1 && sets.turns)) continue;
-              ok = mbar_wait(q_empty(s), (nq[s] & 1u) ^ 1u, abort_flag);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) continue;
-              if (lane == 0) {
-                mbar_expect_tx(q_full(s), (uint32_t)(set_tokens * p.split.block_heads * D * 2));
-                for (int h = 0; h < S::kHalves; ++h)
-                  tma_load_3d(base + s * S::kTile + h * kHalf, &tm_q, q_full(s), h * 64, first_head(p, t.block), t.tok0 + s * set_tokens);
+              if (used[s] & slot) {
+                ok = ok && wait_on(kv_empty(s, g), (parity[s] & slot) != 0, abort_flag);
+                parity[s] ^= slot;
               }
-              ++nq[s];
+              used[s] = reads[s] ? used[s] | slot : used[s] & ~slot;
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const uint32_t landed = kv_full(reads[0] ? (reads[1] ? 2 : 0) : 1, g);
+            if (lane == 0) mbar_expect_tx(landed, bytes);
+            __syncwarp();
+            if (mine >= 0) tma_load_3d(kv_tile(g) + half * kHalf + box * box_rows * 128, which ? &tm_v : &tm_k, landed, half * 64, y, mine);
+            // behind the first keys, which need no other tile to end; a loader for each set's queries
+            if (which == 0 && i == 0 && w.count[loader] > 0 && !(loader == 1 && w.turns)) {
+              ok = wait_on(q_empty(loader), (n_q & 1u) ^ 1u, abort_flag);
+              if (both) ok = ok && wait_on(q_empty_b(), n_b++ & 1u, abort_flag);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              both = loader == 0 && w.turns && w.count[1] > 0;
+              if (lane == 0) {
+                mbar_expect_tx(q_full(loader), (uint32_t)(set_tokens * p.split.block_heads * D * 2));
+                for (int h = 0; h < S::kHalves; ++h)
+                  tma_load_3d(base + loader * S::kTile + h * kHalf, &tm_q, q_full(loader), h * 64, w.head0, w.tok0 + loader * set_tokens);
+              }
+              ++n_q;
             }
           }
         }
-        u += t.take;
-        if (u < hi) next_part(p, t, hi - u);
+        if (!more || !ok) break;
+        w = w2;
       }
+      if (loader == 0 && !cut_here && lane == 0) p.parts.cuts[cta].pieces = 0;
       if (*abort_flag) {  // copies in flight land before shared memory is given back
         const long long t0 = clock64();
         while (clock64() - t0 < 4000000LL) {
         }
       }
-    } else if (warp == 1) {
-      // ------------------------------------------------------------------ matrix products
-      struct Pending {  // a set's output product that waits for its probabilities
-        bool any, first, last, release;
-        uint32_t g;  // its values
-        int keys;    // of them that there are
-      } pend[2] = {};
-      uint32_t g0 = 0, nq[2] = {0, 0}, np[2] = {0, 0}, zeroed = 0xffffffffu;
-      bool ok = true;
-      auto pv = [&](int s) {
-        Pending& w = pend[s];
-        w.any = false;
-        ok = mbar_wait(p_ready(s), np[s]++ & 1u, abort_flag) && mbar_wait(kv_full(w.g), kv_phase(w.g), abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        const uint32_t tile = kv_tile(w.g);
-        if (w.keys < kUnit && zeroed != w.g) {
-          zeroed = w.g;
-          for (int i = lane; i < (kUnit - w.keys) * S::kHalves * 8; i += 32) {
-            const int r = w.keys + i / (S::kHalves * 8), c = i % (S::kHalves * 8);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (c >> 3) * kHalf + r * 128 + (c & 7) * 16), "r"(0) : "memory");
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
+    } else {
+      // ------------------------------------------------------------------ matrix products of set s
+      // The warp stays together and the products are predicated: their descriptors are then made in uniform registers once a tile, where a branch of
+      // one lane would move four words there for every product.
+      const int s = warp >> 1;
+      const uint32_t lead = lane == 0, tm_s = __shfl_sync(0xffffffffu, tmem + (uint32_t)(s * 128), 0), tm_o = __shfl_sync(0xffffffffu, tmem + 256u + (uint32_t)(s * D), 0);
+      uint32_t g = 0, n_q[2] = {0, 0}, n_p = 0, zero_parity = 0;
+      int n_units = 0;
+      uint32_t full_parity[2] = {0, 0};  // a bit for each slot: the phase of the set's kv_full, and of both sets'
+      bool ok = true, any = false;
+      struct {
+        uint32_t g;       // the tile of values that waits for its probabilities
+        int keys;         // of them that there are
+        bool first, last, shared;  // shared: the other set reads it too
+      } w = {};
+      // The sets' steps (an output product with the next scores) go out in turn, unit by unit. Both at once they would mix in the pipe and end side by side, and
+      // both softmax at once would leave the tensor cores idle after; and a set a unit ahead would wait for keys whose place the other still holds. Only an order: a
+      // set that does not get its turn in time goes on without.
+      auto in_turn = [&](int unit) {
         if (lane == 0) {
-          tc_fence_after();
-          // the values' 64-column halves are kHalf bytes apart: the descriptor's leading offset
-          const uint32_t v_lo = ((tile & 0x3FFFFu) >> 4) | ((uint32_t)(kHalf >> 4) << 16);
-#pragma unroll
-          for (int k = 0; k < kUnit / 16; ++k)  // 16 keys: 8 TMEM columns of P, 16 rows of 128 bytes of V
-            umma_f16_ts(tmem + 256u + (uint32_t)(s * D), tmem + (uint32_t)(s * 128 + k * 8), v_lo + (uint32_t)(k * (16 * 128 >> 4)), IDESC_O, !w.first || k != 0);
-          if (w.last) tc_commit(o_done(s));
-          if (w.release) tc_commit(kv_empty(w.g));
+          const long long t0 = clock64();
+          while (passed[1 - s] < unit + s && clock64() - t0 < 20000) {
+          }
         }
         __syncwarp();
       };
-      Part t = part_at(p, prefix, lo, hi - lo);
-      for (long long u = lo; u < hi && ok;) {
-        const Sets sets = sets_of(p, t);
-        for (int i = 0; i < sets.units && ok; ++i) {
-          const uint32_t gk = g0 + 2 * i;
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            if (!ok) break;
-            const bool mine = sets.turns ? (i & 1) == s : i < sets.count[s];
-            // an output product never stays behind a tile's end: the sets' softmax warps wait for one another there
-            if (pend[s].any && (mine || i == 0 || !sets.turns)) pv(s);
-            if (!mine || !ok) continue;
-            const int j = sets.turns ? i >> 1 : i, buf = sets.turns ? 0 : s;
-            ok = mbar_wait(kv_full(gk), kv_phase(gk), abort_flag) && (j > 0 || mbar_wait(q_full(buf), (buf ? nq[1] : nq[0]) & 1u, abort_flag));
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (lane == 0) {
-              tc_fence_after();
-              const uint32_t q_lo = desc_lo(base + buf * S::kTile), k_lo = desc_lo(kv_tile(gk));
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (uint32_t)((k >> 2) * (kHalf >> 4) + (k & 3) * 2);
-                umma_f16(tmem + (uint32_t)(s * 128), q_lo + off, k_lo + off, IDESC_S, k != 0);
-              }
-              tc_commit(s_full(s));
-              if (sets.turns || s == 1) tc_commit(kv_empty(gk));
-              if (sets.turns ? i == sets.units - 1 : j == sets.count[s] - 1) tc_commit(q_empty(buf));
+      auto landed = [&](bool shared, uint32_t g) {
+        const uint32_t slot = 1u << (g % S::kStages), parity = shared ? full_parity[1] : full_parity[0];
+        if (shared) full_parity[1] ^= slot;
+        else full_parity[0] ^= slot;
+        return wait_on(kv_full(shared ? 2 : s, g), (parity & slot) != 0, abort_flag);
+      };
+      auto pv_wait = [&]() {
+        ok = ok && landed(w.shared, w.g) && wait_on(p_ready(s), n_p++ & 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok && w.keys < kUnit) {
+          // what is behind the last key becomes zero, by the first set's warp where both read it
+          if (s == 0 || !w.shared) {
+            const uint32_t tile = kv_tile(w.g);
+#pragma unroll 1
+            for (int i = lane; i < (kUnit - w.keys) * S::kHalves * 8; i += 32) {
+              const int r = w.keys + i / (S::kHalves * 8), c = i % (S::kHalves * 8);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (c >> 3) * kHalf + r * 128 + (c & 7) * 16), "r"(0) : "memory");
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            pend[s] = Pending{true, j == 0, j == sets.count[s] - 1, sets.turns || s == 1, gk + 1, min(kUnit, t.keys - ((int)t.first + i) * kUnit)};
+            if (w.shared && lane == 0) mbar_arrive(v_zero(w.g));
+          } else {
+            const uint32_t slot = 1u << (w.g % S::kStages);
+            ok = __all_sync(0xffffffffu, wait_on(v_zero(w.g), (zero_parity & slot) != 0, abort_flag));
+            zero_parity ^= slot;
           }
         }
-        if (sets.units > 0) {
-          if (sets.turns) ++nq[0];
-          else {
-            nq[0] += sets.count[0] > 0;
-            nq[1] += sets.count[1] > 0;
-          }
-        }
-        g0 += 2 * sets.units;
-        u += t.take;
-        if (u < hi) next_part(p, t, hi - u);
-      }
+      };
+      auto pv_issue = [&]() {
+        any = false;
+        tc_fence_after();
+        // the values' 64-column halves are kHalf bytes apart: the descriptor's leading offset
+        const uint32_t v_lo = __shfl_sync(0xffffffffu, ((kv_tile(w.g) & 0x3FFFFu) >> 4) | ((uint32_t)(kHalf >> 4) << 16), 0);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (ok && pend[s].any) pv(s);
+        for (int k = 0; k < kUnit / 16; ++k)  // 16 keys: 8 TMEM columns of P, 16 rows of 128 bytes of V
+          umma_f16_ts_if(lead, tm_o, tm_s + (uint32_t)(k * 8), v_lo + (uint32_t)(k * (16 * 128 >> 4)), IDESC_O, !w.first || k != 0);
+        if (w.last) tc_commit_if(lead, o_done(s));
+        tc_commit_if(lead, kv_empty(s, w.g));
+      };
+      Work part;
+      for (uint32_t n = 0;; ++n) {
+        const bool more = take_part(n, &part);
+        if (!more) part.units = 1;  // the last output product
+        const int count = s ? part.count[1] : part.count[0], buf = part.turns ? 0 : s;
+        int j = 0;
+        for (int i = 0; i < part.units; ++i, g += 2) {
+          const bool mine = more && (part.turns ? (i & 1) == s : i < count), shared = !part.turns && i < part.count[0];
+          // an output product never stays behind a tile's end: the sets' softmax warps wait for one another there
+          const bool output = any && (mine || i == 0 || !part.turns);
+          if (mine) ok = ok && landed(shared, g) && (j > 0 || wait_on(q_full(buf), (buf ? n_q[1] : n_q[0]) & 1u, abort_flag));
+          if (output) pv_wait();  // the probabilities come last, and are waited for last
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (mine) in_turn(n_units + i);
+          if (output) pv_issue();
+          if (mine) {
+            tc_fence_after();
+            const uint32_t q_lo = __shfl_sync(0xffffffffu, desc_lo(base + buf * S::kTile), 0), k_lo = __shfl_sync(0xffffffffu, desc_lo(kv_tile(g)), 0);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = (uint32_t)((k >> 2) * (kHalf >> 4) + (k & 3) * 2);
+              umma_f16_if(lead, tm_s, q_lo + off, k_lo + off, IDESC_S, k != 0);
+            }
+            tc_commit_if(lead, s_full(s));
+            tc_commit_if(lead, kv_empty(s, g));
+            if (j == count - 1) tc_commit_if(lead, buf == s ? q_empty(s) : q_empty_b());
+            any = true;
+            w.g = g + 1;
+            w.keys = min(kUnit, part.keys - (part.first + i) * kUnit);
+            w.first = j == 0;
+            w.last = j == count - 1;
+            w.shared = shared;
+            ++j;
+          }
+          if (lane == 0) passed[s] = n_units + i + 1;
+        }
+        if (!more || !ok) break;
+        n_units += part.units;
+        n_q[0] += part.count[0] > 0;
+        n_q[1] += !part.turns && part.count[1] > 0;
+      }
     }
   } else if (cta < ctas) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -269,10 +400,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     float* exchange = reinterpret_cast<float*>(smem + S::kExchange) + quad * 16 * 32;
     float2* stats = reinterpret_cast<float2*>(smem + S::kStats) + quad * 32;
     uint32_t n_s = 0, n_o = 0, n_x = 0;
-    bool ok = true, cut_here = false;
+    bool ok = true;
     // what is left to do of the tile before
     struct {
-      bool any, has, whole, join, skip;
+      bool any, has, join, skip;
       int tok0, head0, heads, row0, rows, slot;
       float m, l;
     } w = {};
@@ -281,7 +412,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     auto flush = [&]() {  // whole warp
       w.any = false;
       if (w.has) {
-        if (!all_ok(mbar_wait(o_done(s), n_o & 1u, abort_flag))) return false;
+        if (!all_ok(wait_on(o_done(s), n_o & 1u, abort_flag))) return false;
         ++n_o;
         tc_fence_after();
       }
@@ -289,16 +420,17 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       float scale = w.has ? 1.f : 0.f, other = 0.f;
       if (w.join) {  // both sets hold sums of the same rows: the second's go to the first
         if (s == 1) {
-          if (!all_ok(mbar_wait(ex_empty(quad), (n_x & 1u) ^ 1u, abort_flag))) return false;
+          if (!all_ok(wait_on(ex_empty(quad), (n_x & 1u) ^ 1u, abort_flag))) return false;
           stats[lane] = make_float2(w.m, w.l);
           __syncwarp();
           if (lane == 0) mbar_arrive(ex_full(quad));
           ++n_x;
+#pragma unroll 1
           for (int c = 0; c < D / 16; ++c, ++n_x) {
             uint32_t r[16];
             tmem_ld16_issue(to + (uint32_t)(c * 16), r);
             tmem_ld_wait();
-            if (!all_ok(mbar_wait(ex_empty(quad), (n_x & 1u) ^ 1u, abort_flag))) return false;
+            if (!all_ok(wait_on(ex_empty(quad), (n_x & 1u) ^ 1u, abort_flag))) return false;
 #pragma unroll
             for (int e = 0; e < 16; ++e) exchange[e * 32 + lane] = __uint_as_float(r[e]);
             __syncwarp();
@@ -306,7 +438,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           return true;
         }
-        if (!all_ok(mbar_wait(ex_full(quad), n_x & 1u, abort_flag))) return false;
+        if (!all_ok(wait_on(ex_full(quad), n_x & 1u, abort_flag))) return false;
         const float2 o = stats[lane];
         __syncwarp();
         if (lane == 0) mbar_arrive(ex_empty(quad));
@@ -317,13 +449,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         w.l = w.l * scale + o.y * other;
         w.m = m;
       }
-      const float inv = w.whole ? (w.l == 0.f ? 0.f : 1.f / w.l) : 1.f;
+      const float inv = (w.slot < 0) ? (w.l == 0.f ? 0.f : 1.f / w.l) : 1.f;
       scale *= inv;
       other *= inv;
       // rows of this warp: their number, and where lane / 4 + 8 k lies
       const int rows = w.rows - quad * 32;
       T* dst[4];
-      if (w.whole) {
+      if ((w.slot < 0)) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int r = quad * 32 + k * 8 + (lane >> 2), i = r / p.split.block_heads, h = r % p.split.block_heads;
@@ -332,7 +464,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
       const long long at = (long long)w.slot * kManyRows + w.row0 + row;
       float* part = p.parts.o + at * D;
-      if (!w.whole && row < w.rows) p.parts.ml[at] = make_float2(w.m, w.l);
+      if (w.slot >= 0 && row < w.rows) p.parts.ml[at] = make_float2(w.m, w.l);
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
@@ -348,14 +480,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (w.join) {
 #pragma unroll
           for (int h = 0; h < 2; ++h, ++n_x) {
-            if (!all_ok(mbar_wait(ex_full(quad), n_x & 1u, abort_flag))) return false;
+            if (!all_ok(wait_on(ex_full(quad), n_x & 1u, abort_flag))) return false;
 #pragma unroll
             for (int e = 0; e < 16; ++e) r[h * 16 + e] = __float_as_uint(__uint_as_float(r[h * 16 + e]) + (other == 0.f ? 0.f : exchange[e * 32 + lane] * other));
             __syncwarp();
             if (lane == 0) mbar_arrive(ex_empty(quad));
           }
         }
-        if (w.whole) {  // through shared memory: stores of 64 bytes a row
+        if ((w.slot < 0)) {  // through shared memory: stores of 64 bytes a row
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint4 v;
@@ -383,10 +515,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       return true;
     };
 
-    Part t = part_at(p, prefix, lo, hi - lo);
-    for (long long u = lo; u < hi && ok;) {
-      const Sets sets = sets_of(p, t);
-      const int set = sets.turns ? 0 : s, count = sets.count[s];
+    Work t;
+    for (uint32_t n = 0;; ++n) {
+      const bool more = take_part(n, &t);
+      if (w.any && !flush()) break;
+      if (!more) break;
+      const int set = t.turns ? 0 : s, count = s ? t.count[1] : t.count[0];
       const int set_row0 = set * set_tokens * p.split.block_heads;
       const int rows = min(set_tokens * p.split.block_heads, t.rows - set_row0);  // of the set
       const bool alive = quad * 32 < rows;                                        // whether the warp has any
@@ -396,83 +530,101 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int any_sees = p.split.causal ? min(t.pos0 + set * set_tokens + min(quad * 32 + 31, rows - 1) / p.split.block_heads + 1, t.keys) : t.keys;
       float m_used = -INFINITY, l_run = 0.f;
       for (int j = 0; j < count; ++j, ++n_s) {
-        const int k0 = ((int)t.first + (sets.turns ? 2 * j + s : j)) * kUnit;
-        if (w.any && !flush()) { ok = false; break; }
-        if (!all_ok(mbar_wait(s_full(s), n_s & 1u, abort_flag))) { ok = false; break; }
+        const int k0 = (t.first + (t.turns ? 2 * j + s : j)) * kUnit;
+        if (!all_ok(wait_on(s_full(s), n_s & 1u, abort_flag))) { ok = false; break; }
         if (alive) {
           tc_fence_after();
-          // The scores stay in TMEM until P replaces them, and are taken 32 at a time, the next ones on their way meanwhile (all 128 at once, with P, would not
-          // leave registers for the rest).
-          const int live = max(0, min(any_sees - k0, kUnit) + 31) >> 5;  // chunks of 32 keys that some row of the warp sees
+          const int live = max(0, min(any_sees - k0, kUnit) + 31) >> 5;  // chunks that some row of the warp sees
           const bool edge = k0 + kUnit > all_see;
-          bool need_max = j == 0;
-          float rs0, rs1;
-          uint32_t pk[2][32];
-          while (true) {
-            if (need_max) {
-              float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          uint32_t r[32];
+          auto mask = [&](int c) {
+            if (edge) {
+              const int n = limit - k0 - c * 32;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                if (c >= live) break;
-                uint32_t r[32];
-                tmem_ld32_issue(ts + (uint32_t)(c * 32), r);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!edge || k0 + c * 32 + e < limit) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(r[e]));
-              }
-              const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale);
-              if (j > 0) {  // O holds the tiles before: their products were complete before these scores were
-                const float corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
-                l_run *= corr;
+              for (int e = 0; e < 32; ++e)
+                if (e >= n) r[e] = 0xff800000u;
+            }
+          };
+          if (j == 0) {
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                  uint32_t r[32];
-                  tmem_ld32_issue(to + (uint32_t)(c * 32), r);
+            for (int c = 0; c < live; ++c) {
+              tmem_ld32_issue(ts + (uint32_t)(c * 32), r);
+              tmem_ld_wait();
+              mask(c);
+              float top = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) top = fmaxf(fmaxf(top, __uint_as_float(r[e])), __uint_as_float(r[e + 1]));
+              m_used = fmaxf(m_used, top * p.scale);
+            }
+          }
+          // 32 scores at a time, the next on their way meanwhile; their probabilities replace scores that have been read. The loop is one chunk long on purpose:
+          // the instruction cache is the other warps' too, and with the tile unrolled they stood still for their own (16 products 3500 cycles in place of 1250).
+          float l0 = 0.f, l1 = 0.f;
+          tmem_ld32_issue(ts, r);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+            tmem_ld_wait();
+            if (c < live) {  // warp-uniform
+              mask(c);
+              const float m_sub = m_used == -INFINITY ? 0.f : m_used;
+              float x[32], s0 = 0.f, s1 = 0.f;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] = fmaf(__uint_as_float(r[e]), p.scale, -m_sub);
+              if (c < 3) tmem_ld32_issue(ts + (uint32_t)((c + 1) * 32), r);
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                const float a0 = ex2(x[e]), a1 = ex2(x[e + 1]), a2 = ex2(x[e + 2]), a3 = (e & 4) ? ex2_poly(x[e + 3]) : ex2(x[e + 3]);
+                s0 += a0 + a1;
+                s1 += a2 + a3;
+                pk[e >> 1] = pack2<T>(a0, a1);
+                pk[(e >> 1) + 1] = pack2<T>(a2, a3);
+              }
+              if (__builtin_expect(__any_sync(0xffffffffu, row < rows && !(s0 + s1 < kSumLimit)), 0)) {
+                // A score far above the reference (or no number): everything so far is brought to a new one, and these are made again. (O holds the tiles before:
+                // their products were complete before these scores were.)
+                float top = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
+                const float m_new = fmaxf(m_used, m_sub + top), corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
+                const float down = m_sub - (m_new == -INFINITY ? 0.f : m_new);
+                m_used = m_new;
+                l_run *= corr;
+                l0 *= corr;
+                l1 *= corr;
+                tmem_st_wait();
+                tmem_ld_wait();
+#pragma unroll 1
+                for (int i = j > 0 ? 0 : D / 16; i < D / 16 + c; ++i) {
+                  const uint32_t at = i < D / 16 ? to + (uint32_t)(i * 16) : ts + (uint32_t)((i - D / 16) * 16);
+                  tmem_ld16_issue(at, pk);
                   tmem_ld_wait();
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
-                  tmem_st32(to + (uint32_t)(c * 32), r);
+                  for (int e = 0; e < 16; ++e) {
+                    const float2 f = unpack2<T>(pk[e]);
+                    pk[e] = i < D / 16 ? __float_as_uint(__uint_as_float(pk[e]) * corr) : pack2<T>(f.x * corr, f.y * corr);
+                  }
+                  tmem_st16(at, pk);
+                }
+                tmem_st_wait();
+                s0 = s1 = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const float a0 = ex2(x[2 * e] + down), a1 = ex2(x[2 * e + 1] + down);
+                  s0 += a0;
+                  s1 += a1;
+                  pk[e] = pack2<T>(a0, a1);
                 }
               }
-              m_used = m_new;
+              l0 += s0;
+              l1 += s1;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) pk[e] = 0u;
             }
-            const float m_sub = m_used == -INFINITY ? 0.f : m_used;
-            rs0 = rs1 = 0.f;
-            uint32_t sr[2][32];
-            tmem_ld32_issue(ts, sr[0]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t* dst = &pk[c >> 1][(c & 1) * 16];
-              uint32_t* r = sr[c & 1];
-              tmem_ld_wait();
-              if (c < 3) tmem_ld32_issue(ts + (uint32_t)((c + 1) * 32), sr[(c + 1) & 1]);
-              if (c < live) {  // warp-uniform
-                if (edge) {
-#pragma unroll
-                  for (int e = 0; e < 32; ++e)
-                    if (k0 + c * 32 + e >= limit) r[e] = 0xff800000u;
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                  const float a0 = ex2(fmaf(__uint_as_float(r[e]), p.scale, -m_sub)), a1 = ex2(fmaf(__uint_as_float(r[e + 1]), p.scale, -m_sub));
-                  const float a2 = ex2(fmaf(__uint_as_float(r[e + 2]), p.scale, -m_sub)), a3 = ex2(fmaf(__uint_as_float(r[e + 3]), p.scale, -m_sub));
-                  rs0 += a0 + a1;
-                  rs1 += a2 + a3;
-                  dst[e >> 1] = pack2<T>(a0, a1);
-                  dst[(e >> 1) + 1] = pack2<T>(a2, a3);
-                }
-              } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) dst[e] = 0u;
-              }
-            }
-            if (need_max || !__any_sync(0xffffffffu, row < rows && !(rs0 + rs1 < kRowSumLimit))) break;
-            need_max = true;  // a score far above the reference: once more, against its true maximum
+            tmem_st16(ts + (uint32_t)(c * 16), pk);
           }
-          l_run += rs0 + rs1;
-          tmem_st32(ts, pk[0]);
-          tmem_st32(ts + 32u, pk[1]);
+          l_run += l0 + l1;
           tmem_st_wait();
           tc_fence_before();
         }
@@ -480,31 +632,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (lane == 0) mbar_arrive(p_ready(s));
       }
       if (!ok) break;
-      // what becomes of the tile. A set whose rows all lie before the stretch's keys has no sums, but says so to whoever joins the parts.
-      const bool whole = t.take == t.units;
-      if (w.any && !flush()) { ok = false; break; }  // (it had no tile of its own to do that in)
-      w.any = count > 0 || !sets.turns || s == 0;
+      // what becomes of the tile. A set whose rows all lie before the part's keys has no sums, but says so to whoever joins the parts.
+      w.any = count > 0 || !t.turns || s == 0;
       w.has = count > 0;
-      w.join = sets.turns && sets.count[1] > 0;
-      w.whole = whole;
+      w.join = t.turns && t.count[1] > 0;
       w.skip = !alive;
       w.tok0 = t.tok0 + set * set_tokens;
-      w.head0 = first_head(p, t.block);
-      w.heads = heads_of(p, t.block);
+      w.head0 = t.head0;
+      w.heads = t.heads;
       w.row0 = set_row0;
       w.rows = rows;
-      w.slot = 2 * cta + (u == lo ? 0 : 1);
+      w.slot = t.slot;
       w.m = m_used;
       w.l = l_run;
-      if (!whole && t.first == 0) {
-        cut_here = true;
-        if (threadIdx.x == 128) p.parts.cuts[cta] = cut_of(p, t, u, total, cta, ctas, w.slot);
-      }
-      u += t.take;
-      if (u < hi) next_part(p, t, hi - u);
     }
-    if (ok && w.any) flush();
-    if (!cut_here && threadIdx.x == 128) p.parts.cuts[cta].pieces = 0;
   }
 
   tc_fence_before();
@@ -520,13 +661,7 @@ template <typename T, int D>
 int launch(ttb_ctx* ctx, const ttb_paged_kv* kv, int64_t heads, const Params& p) {
   using S = Shape<D>;
   CUtensorMap tm_q, tm_k, tm_v;
-  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-  const uint32_t box_rows = (uint32_t)std::min<int64_t>(kv->page_tokens, kUnit);
-  const uint64_t pages = (uint64_t)kv->pages, rows = (uint64_t)(kv->kv_heads * kv->page_tokens), stride = (uint64_t)kv->page_stride;
-  if (!encode_tile_map_3d(&tm_q, p.q, bf16, (uint64_t)p.s.tokens, (uint64_t)heads, D, (uint64_t)p.ldq, D, (uint32_t)(p.split.tile_tokens / 2),
-                          (uint32_t)p.split.block_heads) ||
-      !encode_tile_map_3d(&tm_k, kv->keys, bf16, pages, rows, D, stride, D, 1, box_rows) ||
-      !encode_tile_map_3d(&tm_v, kv->values, bf16, pages, rows, D, stride, D, 1, box_rows))
+  if (!encode_maps(kv, std::is_same<T, __nv_bfloat16>::value, heads, p, p.split.tile_tokens / 2, &tm_q, &tm_k, &tm_v))
     return fail(ctx, TTB_ERR_CUDA, "paged_attention: a tensor map was refused");
   static bool configured[64] = {};
   const int dev = ctx->device < 64 ? ctx->device : 63;
