@@ -4,8 +4,8 @@
 // One CTA an SM walks its stretch of the line (ttb_paged_rules.cuh). A tile is two sets of 128 query rows (tokens x heads of a key head) that share every key and value
 // tile of 128 tokens, so that 64 KB of them (heads of 128) feed 2 x 128 rows: with a set alone the tensor cores would want them twice as fast. A tile whose rows all
 // fit one set (a few tokens) puts them into both: the sets take the key tiles in turn and are joined at the tile's end, so that one's products still run beside the other's softmax.
-//   warps 0, 2  : loads - a lane for each box (a page, or 128 keys) and half of a head, half of them a warp's (a copy takes its thread some 60 cycles to issue,
-//                 one lane after the other): queries, and keys and values in turn through one ring
+//   warps 0, 2  : loads - warp 0 queries and keys, warp 2 values, each as soon as its ring (of two or four tiles) has room; a lane for each box (a page, or 128 tokens)
+//                 and half of a head
 //   warps 1, 3  : matrix products of a set each - S = Q K^T (128 x 128, fp32 in TMEM), O += P V with P in TMEM over the scores it came from, V as it lies, in
 //                 the order QK(0), PV(0), QK(1), PV(1), ...; everything a product waits for but the softmax is a barrier poll. Rows of V behind the last key are
 //                 set to zero here: a probability of zero would not undo what the page happens to hold.
@@ -24,7 +24,7 @@ using namespace ttb::sm100;
 
 namespace {
 
-constexpr int kThreads = 384, kLoaders = 2;
+constexpr int kThreads = 384;
 constexpr int kSet = kManyRows / 2;      // rows of a set
 constexpr int kHalf = kUnit * 128;       // bytes of 128 rows of 64 elements
 constexpr uint32_t kTmemCols = 512;
@@ -150,7 +150,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       int count = 1;
       if (k == 6 || k == 7) count = 4;                                                            // p_ready: the set's four warps
       if (k >= 19 + kRingWorks && k < 19 + 2 * kRingWorks) count = kThreads / 32 - 1;             // part_empty: all warps but the one that fills it
-      if (k >= S::kFirstSlotBar && k < S::kFirstSlotBar + 3 * S::kStages) count = kLoaders;       // kv_full
       mbar_init(bar(k), count);
     }
     *abort_flag = 0;
@@ -190,8 +189,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // ------------------------------------------------------------------ loads
       const int loader = warp >> 1;
       const int page_tokens = 1 << p.s.page_shift, box_rows = min(page_tokens, kUnit);
-      const int at = lane * kLoaders + loader, box = at / S::kHalves, half = at % S::kHalves;
-      uint32_t g = 0, n_q = 0, n_b = 0, n = 0;
+      const int box = lane / S::kHalves, half = lane % S::kHalves;
+      uint32_t g = loader, n_q[2] = {0, 0}, n_b = 0, n = 0;  // g: tile, keys even and values odd
       uint32_t used[2] = {0, 0}, parity[2] = {0, 0};  // a bit for each slot: whether the set reads what is there, and the phase of its kv_empty
       bool ok = true, both = false;                   // both: the second set reads the first queries' buffer too
       // The first loader works the parts out, one ahead of its own loads.
@@ -239,37 +238,38 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           page = i + 1 < w.units ? page_at(w, i + 1) : more ? page_at(w2, 0) : 0;
           const uint32_t bytes = (uint32_t)(__popc(__ballot_sync(0xffffffffu, mine >= 0)) * box_rows * 128);
           const bool reads[2] = {w.turns ? (i & 1) == 0 : i < w.count[0], w.turns ? (i & 1) == 1 : true};
-#pragma unroll 1
-          for (int which = 0; which < 2; ++which, ++g) {  // keys, values
-            const uint32_t slot = 1u << (g % S::kStages);
+          const uint32_t slot = 1u << (g % S::kStages);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              if (used[s] & slot) {
-                ok = ok && wait_on(kv_empty(s, g), (parity[s] & slot) != 0, abort_flag);
-                parity[s] ^= slot;
-              }
-              used[s] = reads[s] ? used[s] | slot : used[s] & ~slot;
+          for (int s = 0; s < 2; ++s) {
+            if (used[s] & slot) {
+              ok = ok && wait_on(kv_empty(s, g), (parity[s] & slot) != 0, abort_flag);
+              parity[s] ^= slot;
+            }
+            used[s] = reads[s] ? used[s] | slot : used[s] & ~slot;
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t landed = kv_full(reads[0] ? (reads[1] ? 2 : 0) : 1, g);
+          if (lane == 0) mbar_expect_tx(landed, bytes);
+          __syncwarp();
+          if (mine >= 0) tma_load_3d(kv_tile(g) + half * kHalf + box * box_rows * 128, loader ? &tm_v : &tm_k, landed, half * 64, y, mine);
+          g += 2;
+          // the queries go behind the first keys, which need no other tile to end
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (!ok || loader || i > 0 || w.count[s] == 0 || (s == 1 && w.turns)) continue;
+            ok = wait_on(q_empty(s), (n_q[s] & 1u) ^ 1u, abort_flag);
+            if (s == 0) {
+              if (both) ok = ok && wait_on(q_empty_b(), n_b++ & 1u, abort_flag);
+              both = w.turns && w.count[1] > 0;
             }
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            const uint32_t landed = kv_full(reads[0] ? (reads[1] ? 2 : 0) : 1, g);
-            if (lane == 0) mbar_expect_tx(landed, bytes);
-            __syncwarp();
-            if (mine >= 0) tma_load_3d(kv_tile(g) + half * kHalf + box * box_rows * 128, which ? &tm_v : &tm_k, landed, half * 64, y, mine);
-            // behind the first keys, which need no other tile to end; a loader for each set's queries
-            if (which == 0 && i == 0 && w.count[loader] > 0 && !(loader == 1 && w.turns)) {
-              ok = wait_on(q_empty(loader), (n_q & 1u) ^ 1u, abort_flag);
-              if (both) ok = ok && wait_on(q_empty_b(), n_b++ & 1u, abort_flag);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              both = loader == 0 && w.turns && w.count[1] > 0;
-              if (lane == 0) {
-                mbar_expect_tx(q_full(loader), (uint32_t)(set_tokens * p.split.block_heads * D * 2));
-                for (int h = 0; h < S::kHalves; ++h)
-                  tma_load_3d(base + loader * S::kTile + h * kHalf, &tm_q, q_full(loader), h * 64, w.head0, w.tok0 + loader * set_tokens);
-              }
-              ++n_q;
+            if (ok && lane == 0) {
+              mbar_expect_tx(q_full(s), (uint32_t)(set_tokens * p.split.block_heads * D * 2));
+              for (int h = 0; h < S::kHalves; ++h)
+                tma_load_3d(base + s * S::kTile + h * kHalf, &tm_q, q_full(s), h * 64, w.head0, w.tok0 + s * set_tokens);
             }
+            ++n_q[s];
           }
         }
         if (!more || !ok) break;
