@@ -7,8 +7,7 @@
 //   warps 0, 2  : loads - warp 0 queries and keys, warp 2 values, each as soon as its ring (of two or four tiles) has room; a lane for each box (a page, or 128 tokens)
 //                 and half of a head
 //   warps 1, 3  : matrix products of a set each - S = Q K^T (128 x 128, fp32 in TMEM), O += P V with P in TMEM over the scores it came from, V as it lies, in
-//                 the order QK(0), PV(0), QK(1), PV(1), ...; everything a product waits for but the softmax is a barrier poll. Rows of V behind the last key are
-//                 set to zero here: a probability of zero would not undo what the page happens to hold.
+//                 the order QK(0), PV(0), QK(1), PV(1), ...; everything a product waits for but the softmax is a barrier poll
 //   warps 4..11 : softmax, a warpgroup a set, a row a thread: scores from TMEM, exp2 with the scale folded in, P back to TMEM in 16 bits. The row's reference is the maximum of
 //                 its first tile; it is raised (and O rescaled) only where the sum of 32 probabilities passes 2^15: the division by the sum makes the result independent of it.
 // A tile's output is written while the next one's first scores are made. Every wait is bounded.
@@ -58,8 +57,8 @@ template <int D> struct Shape {
   static constexpr int kScratch = kPrefix + (kMaxSequences + 1) * 8;
   static constexpr int kWorks = kScratch + kThreads / 32 * 8;
   static constexpr int kBars = kWorks + kRingWorks * (int)sizeof(Work);
-  static constexpr int kFirstSlotBar = 19 + 2 * kRingWorks;
-  static constexpr int kNumBars = kFirstSlotBar + 6 * kStages;
+  static constexpr int kFirstSlotBar = 20 + 2 * kRingWorks;
+  static constexpr int kNumBars = kFirstSlotBar + 5 * kStages;
   static constexpr int kBytes = kBars + kNumBars * 8 + 16;
 };
 
@@ -74,15 +73,32 @@ __device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile 
   return false;
 }
 
-// 2^x on the fp32 pipe, for one probability in eight, which the special-function unit is the limit of: 2^n * 2^f with n the nearest whole number, and 2^f on [-1/2, 1/2] by
-// a polynomial fitted to the least relative error (2^-18.5, far below P's rounding). A score that is no number or far above the reference gives 2^127, which the row sum tells.
-__device__ __forceinline__ float ex2_poly(float x) {
-  x = fmaxf(fminf(x, 127.f), -126.f);
-  const float n = x + 12582912.f;  // 3 * 2^22: the sum's last bit is one
-  const float f = x - (n - 12582912.f);
-  const float y = fmaf(fmaf(fmaf(fmaf(0.009570102207362652f, f, 0.05591786280274391f), f, 0.240247443318367f), f, 0.6931217908859253f), f, 0.9999992847442627f);
-  return __int_as_float(__float_as_int(y) + (__float_as_int(n) << 23));
+// Two fp32 operations an instruction.
+__device__ __forceinline__ void fma2(uint32_t a0, uint32_t a1, float b, float c, float* d0, float* d1) {
+  asm("{\n"
+      ".reg .b64 a, b, c, d;\n"
+      "mov.b64 a, {%2, %3};\n"
+      "mov.b64 b, {%4, %4};\n"
+      "mov.b64 c, {%5, %5};\n"
+      "fma.rn.f32x2 d, a, b, c;\n"
+      "mov.b64 {%0, %1}, d;\n"
+      "}\n"
+      : "=f"(*d0), "=f"(*d1)
+      : "r"(a0), "r"(a1), "f"(b), "f"(c));
 }
+__device__ __forceinline__ unsigned long long add2(unsigned long long s, float a0, float a1) {
+  unsigned long long d;
+  asm("{\n"
+      ".reg .b64 a;\n"
+      "mov.b64 a, {%2, %3};\n"
+      "add.rn.f32x2 %0, %1, a;\n"
+      "}\n"
+      : "=l"(d)
+      : "l"(s), "f"(a0), "f"(a1));
+  return d;
+}
+__device__ __forceinline__ float lo2(unsigned long long s) { return __uint_as_float((uint32_t)s); }
+__device__ __forceinline__ float hi2(unsigned long long s) { return __uint_as_float((uint32_t)(s >> 32)); }
 
 __device__ __forceinline__ Work work_of(const Params& p, const Part& t, int slot) {
   const int tokens = p.split.tile_tokens / 2;  // of a set
@@ -133,11 +149,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   auto q_empty_b = [&]() { return bar(18); };  // the first queries' buffer, by the second set where both read it
   // A tile has landed for the first set, the second, or both (2). A wait tells a phase from the next and not from the one after: a barrier's waiters have to
   // wait for its every phase, so that a tile that one set passes over is not told to it.
-  auto part_full = [&](uint32_t n) { return bar(19 + (int)(n % kRingWorks)); };
-  auto part_empty = [&](uint32_t n) { return bar(19 + kRingWorks + (int)(n % kRingWorks)); };
+  const uint32_t v_tail = bar(19);  // values that end inside their tile, for the warp that loads them
+  auto part_full = [&](uint32_t n) { return bar(20 + (int)(n % kRingWorks)); };
+  auto part_empty = [&](uint32_t n) { return bar(20 + kRingWorks + (int)(n % kRingWorks)); };
   auto kv_full = [&](int f, uint32_t g) { return bar(S::kFirstSlotBar + f * S::kStages + (int)(g % S::kStages)); };
   auto kv_empty = [&](int s, uint32_t g) { return bar(S::kFirstSlotBar + (3 + s) * S::kStages + (int)(g % S::kStages)); };  // by the sets that read the tile
-  auto v_zero = [&](uint32_t g) { return bar(S::kFirstSlotBar + 5 * S::kStages + (int)(g % S::kStages)); };
   auto kv_tile = [&](uint32_t g) { return base + S::kRing + (g % S::kStages) * S::kTile; };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -149,7 +165,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     for (int k = 0; k < S::kNumBars; ++k) {
       int count = 1;
       if (k == 6 || k == 7) count = 4;                                                            // p_ready: the set's four warps
-      if (k >= 19 + kRingWorks && k < 19 + 2 * kRingWorks) count = kThreads / 32 - 1;             // part_empty: all warps but the one that fills it
+      if (k >= 20 + kRingWorks && k < 20 + 2 * kRingWorks) count = kThreads / 32 - 1;             // part_empty: all warps but the one that fills it
       mbar_init(bar(k), count);
     }
     *abort_flag = 0;
@@ -190,7 +206,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const int loader = warp >> 1;
       const int page_tokens = 1 << p.s.page_shift, box_rows = min(page_tokens, kUnit);
       const int box = lane / S::kHalves, half = lane % S::kHalves;
-      uint32_t g = loader, n_q[2] = {0, 0}, n_b = 0, n = 0;  // g: tile, keys even and values odd
+      uint32_t g = loader, n_q[2] = {0, 0}, n_b = 0, n_tail = 0, n = 0;  // g: tile, keys even and values odd
       uint32_t used[2] = {0, 0}, parity[2] = {0, 0};  // a bit for each slot: whether the set reads what is there, and the phase of its kv_empty
       bool ok = true, both = false;                   // both: the second set reads the first queries' buffer too
       // The first loader works the parts out, one ahead of its own loads.
@@ -249,10 +265,25 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          const uint32_t landed = kv_full(reads[0] ? (reads[1] ? 2 : 0) : 1, g);
+          // Values behind the last key become zero, whatever the page happens to hold there: a probability of zero would not undo what is not finite.
+          const int there = w.keys - (w.first + i) * kUnit;
+          const bool tail = loader && there < kUnit;
+          const uint32_t full = kv_full(reads[0] ? (reads[1] ? 2 : 0) : 1, g), landed = tail ? v_tail : full;
           if (lane == 0) mbar_expect_tx(landed, bytes);
           __syncwarp();
           if (mine >= 0) tma_load_3d(kv_tile(g) + half * kHalf + box * box_rows * 128, loader ? &tm_v : &tm_k, landed, half * 64, y, mine);
+          if (tail) {
+            ok = __all_sync(0xffffffffu, wait_on(v_tail, n_tail++ & 1u, abort_flag));
+            if (!ok) break;
+#pragma unroll 1
+            for (int c = lane; c < (kUnit - there) * S::kHalves * 8; c += 32) {
+              const int r = there + c / (S::kHalves * 8), col = c % (S::kHalves * 8);
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(kv_tile(g) + (col >> 3) * kHalf + r * 128 + (col & 7) * 16), "r"(0) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+          }
           g += 2;
           // the queries go behind the first keys, which need no other tile to end
 #pragma unroll
@@ -283,111 +314,85 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
     } else {
       // ------------------------------------------------------------------ matrix products of set s
-      // The warp stays together and the products are predicated: their descriptors are then made in uniform registers once a tile, where a branch of
-      // one lane would move four words there for every product.
+      // One lane, and few instructions between the arrival of the probabilities and the products: beside the softmax they come from the second-level instruction
+      // cache every time.
       const int s = warp >> 1;
-      const uint32_t lead = lane == 0, tm_s = __shfl_sync(0xffffffffu, tmem + (uint32_t)(s * 128), 0), tm_o = __shfl_sync(0xffffffffu, tmem + 256u + (uint32_t)(s * D), 0);
-      uint32_t g = 0, n_q[2] = {0, 0}, n_p = 0, zero_parity = 0;
-      int n_units = 0;
-      uint32_t full_parity[2] = {0, 0};  // a bit for each slot: the phase of the set's kv_full, and of both sets'
-      bool ok = true, any = false;
-      struct {
-        uint32_t g;       // the tile of values that waits for its probabilities
-        int keys;         // of them that there are
-        bool first, last, shared;  // shared: the other set reads it too
-      } w = {};
-      // The sets' steps (an output product with the next scores) go out in turn, unit by unit. Both at once they would mix in the pipe and end side by side, and
-      // both softmax at once would leave the tensor cores idle after; and a set a unit ahead would wait for keys whose place the other still holds. Only an order: a
-      // set that does not get its turn in time goes on without.
-      auto in_turn = [&](int unit) {
-        if (lane == 0) {
-          const long long t0 = clock64();
-          while (passed[1 - s] < unit + s && clock64() - t0 < 20000) {
-          }
-        }
-        __syncwarp();
-      };
-      auto landed = [&](bool shared, uint32_t g) {
-        const uint32_t slot = 1u << (g % S::kStages), parity = shared ? full_parity[1] : full_parity[0];
-        if (shared) full_parity[1] ^= slot;
-        else full_parity[0] ^= slot;
-        return wait_on(kv_full(shared ? 2 : s, g), (parity & slot) != 0, abort_flag);
-      };
-      auto pv_wait = [&]() {
-        ok = ok && landed(w.shared, w.g) && wait_on(p_ready(s), n_p++ & 1u, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && w.keys < kUnit) {
-          // what is behind the last key becomes zero, by the first set's warp where both read it
-          if (s == 0 || !w.shared) {
-            const uint32_t tile = kv_tile(w.g);
+      if (lane == 0) {
+        const uint32_t tm_s = tmem + (uint32_t)(s * 128), tm_o = tmem + 256u + (uint32_t)(s * D);
+        uint32_t g = 0, n_q[2] = {0, 0}, n_p = 0, w_g = 0;  // w_g: the tile of values that waits for its probabilities
+        uint32_t full_parity[2] = {0, 0};                   // a bit for each slot: the phase of the set's kv_full, and of both sets'
+        int n_units = 0;
+        bool ok = true, any = false, w_first = false, w_last = false, w_shared = false;
+        auto landed = [&](bool shared, uint32_t g) {
+          const uint32_t slot = 1u << (g % S::kStages), parity = shared ? full_parity[1] : full_parity[0];
+          if (shared) full_parity[1] ^= slot;
+          else full_parity[0] ^= slot;
+          return wait_on(kv_full(shared ? 2 : s, g), (parity & slot) != 0, abort_flag);
+        };
+        for (uint32_t n = 0;; ++n) {
+          if (!wait_on(part_full(n), (n / kRingWorks) & 1u, abort_flag)) break;
+          const Work& part = works[n % kRingWorks];
+          const bool more = part.units >= 0, turns = part.turns;
+          const int units = more ? part.units : 1, count0 = part.count[0], count1 = part.count[1], count = s ? count1 : count0, buf = turns ? 0 : s;
+          mbar_arrive(part_empty(n));
+          int j = 0;
+          for (int i = 0; i < units; ++i, g += 2) {  // (behind the last part: its last output product)
+            const bool mine = more && (turns ? (i & 1) == s : i < count), shared = !turns && i < count0;
+            // an output product never stays behind a tile's end: the sets' softmax warps wait for one another there
+            const bool output = any && (mine || i == 0 || !turns);
+            if (mine) ok = landed(shared, g) && (j > 0 || wait_on(q_full(buf), (buf ? n_q[1] : n_q[0]) & 1u, abort_flag));
+            if (ok && output) ok = landed(w_shared, w_g) && wait_on(p_ready(s), n_p++ & 1u, abort_flag);  // the probabilities come last
+            if (!ok) break;
+            if (mine) {
+              // The sets' steps (an output product with the next scores) go out in turn, unit by unit. Both at once they would mix in the pipe and end side by side,
+              // and both softmax at once would leave the tensor cores idle after; and a set a unit ahead would wait for keys whose place the other still holds. Only
+              // an order: a set that does not get its turn in time goes on without.
+              const int unit = n_units + i;
 #pragma unroll 1
-            for (int i = lane; i < (kUnit - w.keys) * S::kHalves * 8; i += 32) {
-              const int r = w.keys + i / (S::kHalves * 8), c = i % (S::kHalves * 8);
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (c >> 3) * kHalf + r * 128 + (c & 7) * 16), "r"(0) : "memory");
+              for (int tries = 0; passed[1 - s] < unit + s && tries < 500; ++tries) {
+              }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (w.shared && lane == 0) mbar_arrive(v_zero(w.g));
-          } else {
-            const uint32_t slot = 1u << (w.g % S::kStages);
-            ok = __all_sync(0xffffffffu, wait_on(v_zero(w.g), (zero_parity & slot) != 0, abort_flag));
-            zero_parity ^= slot;
-          }
-        }
-      };
-      auto pv_issue = [&]() {
-        any = false;
-        tc_fence_after();
-        // the values' 64-column halves are kHalf bytes apart: the descriptor's leading offset
-        const uint32_t v_lo = __shfl_sync(0xffffffffu, ((kv_tile(w.g) & 0x3FFFFu) >> 4) | ((uint32_t)(kHalf >> 4) << 16), 0);
-#pragma unroll
-        for (int k = 0; k < kUnit / 16; ++k)  // 16 keys: 8 TMEM columns of P, 16 rows of 128 bytes of V
-          umma_f16_ts_if(lead, tm_o, tm_s + (uint32_t)(k * 8), v_lo + (uint32_t)(k * (16 * 128 >> 4)), IDESC_O, !w.first || k != 0);
-        if (w.last) tc_commit_if(lead, o_done(s));
-        tc_commit_if(lead, kv_empty(s, w.g));
-      };
-      Work part;
-      for (uint32_t n = 0;; ++n) {
-        const bool more = take_part(n, &part);
-        if (!more) part.units = 1;  // the last output product
-        const int count = s ? part.count[1] : part.count[0], buf = part.turns ? 0 : s;
-        int j = 0;
-        for (int i = 0; i < part.units; ++i, g += 2) {
-          const bool mine = more && (part.turns ? (i & 1) == s : i < count), shared = !part.turns && i < part.count[0];
-          // an output product never stays behind a tile's end: the sets' softmax warps wait for one another there
-          const bool output = any && (mine || i == 0 || !part.turns);
-          if (mine) ok = ok && landed(shared, g) && (j > 0 || wait_on(q_full(buf), (buf ? n_q[1] : n_q[0]) & 1u, abort_flag));
-          if (output) pv_wait();  // the probabilities come last, and are waited for last
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (mine) in_turn(n_units + i);
-          if (output) pv_issue();
-          if (mine) {
             tc_fence_after();
-            const uint32_t q_lo = __shfl_sync(0xffffffffu, desc_lo(base + buf * S::kTile), 0), k_lo = __shfl_sync(0xffffffffu, desc_lo(kv_tile(g)), 0);
+            if (output) {
+              // the values' 64-column halves are kHalf bytes apart: the descriptor's leading offset
+              const uint32_t v_lo = ((kv_tile(w_g) & 0x3FFFFu) >> 4) | ((uint32_t)(kHalf >> 4) << 16);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t off = (uint32_t)((k >> 2) * (kHalf >> 4) + (k & 3) * 2);
-              umma_f16_if(lead, tm_s, q_lo + off, k_lo + off, IDESC_S, k != 0);
+              for (int k = 0; k < kUnit / 16; ++k)  // 16 keys: 8 TMEM columns of P, 16 rows of 128 bytes of V
+                umma_f16_ts(tm_o, tm_s + (uint32_t)(k * 8), v_lo + (uint32_t)(k * (16 * 128 >> 4)), IDESC_O, !w_first || k != 0);
             }
-            tc_commit_if(lead, s_full(s));
-            tc_commit_if(lead, kv_empty(s, g));
-            if (j == count - 1) tc_commit_if(lead, buf == s ? q_empty(s) : q_empty_b());
-            any = true;
-            w.g = g + 1;
-            w.keys = min(kUnit, part.keys - (part.first + i) * kUnit);
-            w.first = j == 0;
-            w.last = j == count - 1;
-            w.shared = shared;
-            ++j;
+            if (mine) {
+              const uint32_t q_lo = desc_lo(base + buf * S::kTile), k_lo = desc_lo(kv_tile(g));
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (uint32_t)((k >> 2) * (kHalf >> 4) + (k & 3) * 2);
+                umma_f16(tm_s, q_lo + off, k_lo + off, IDESC_S, k != 0);
+              }
+              tc_commit(s_full(s));
+            }
+            passed[s] = n_units + i + 1;
+            if (output) {
+              if (w_last) tc_commit(o_done(s));
+              tc_commit(kv_empty(s, w_g));
+              any = false;
+            }
+            if (mine) {
+              tc_commit(kv_empty(s, g));
+              if (j == count - 1) tc_commit(buf == s ? q_empty(s) : q_empty_b());
+              any = true;
+              w_g = g + 1;
+              w_first = j == 0;
+              w_last = j == count - 1;
+              w_shared = shared;
+              ++j;
+            }
           }
-          if (lane == 0) passed[s] = n_units + i + 1;
+          if (!more || !ok) break;
+          n_units += units;
+          n_q[0] += count0 > 0;
+          n_q[1] += !turns && count1 > 0;
         }
-        if (!more || !ok) break;
-        n_units += part.units;
-        n_q[0] += part.count[0] > 0;
-        n_q[1] += !part.turns && part.count[1] > 0;
       }
+      __syncwarp();
     }
   } else if (cta < ctas) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -557,72 +562,106 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               m_used = fmaxf(m_used, top * p.scale);
             }
           }
-          // 32 scores at a time, the next on their way meanwhile; their probabilities replace scores that have been read. The loop is one chunk long on purpose:
-          // the instruction cache is the other warps' too, and with the tile unrolled they stood still for their own (16 products 3500 cycles in place of 1250).
+          // A tile that every row sees the whole of, against a reference that an earlier one gave: straight through, P kept until its sum says that the reference still
+          // holds. Short code, since the instruction cache is the other warps' too (with masks and rescaling in it 16 products took 3500 cycles in place of 1250).
           float l0 = 0.f, l1 = 0.f;
-          tmem_ld32_issue(ts, r);
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-            tmem_ld_wait();
-            if (c < live) {  // warp-uniform
-              mask(c);
-              const float m_sub = m_used == -INFINITY ? 0.f : m_used;
-              float x[32], s0 = 0.f, s1 = 0.f;
+          bool done = false;
+          if (j > 0 && !edge) {
+            uint32_t pk[2][32];
+            unsigned long long sum = 0, sum2 = 0;
+            const float m_sub = m_used == -INFINITY ? 0.f : m_used;
+            tmem_ld32_issue(ts, r);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = fmaf(__uint_as_float(r[e]), p.scale, -m_sub);
+            for (int c = 0; c < 4; ++c) {
+              float x[32];
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) fma2(r[e], r[e + 1], p.scale, -m_sub, &x[e], &x[e + 1]);
               if (c < 3) tmem_ld32_issue(ts + (uint32_t)((c + 1) * 32), r);
 #pragma unroll
               for (int e = 0; e < 32; e += 4) {
-                const float a0 = ex2(x[e]), a1 = ex2(x[e + 1]), a2 = ex2(x[e + 2]), a3 = (e & 4) ? ex2_poly(x[e + 3]) : ex2(x[e + 3]);
-                s0 += a0 + a1;
-                s1 += a2 + a3;
-                pk[e >> 1] = pack2<T>(a0, a1);
-                pk[(e >> 1) + 1] = pack2<T>(a2, a3);
+                const float a0 = ex2(x[e]), a1 = ex2(x[e + 1]), a2 = ex2(x[e + 2]), a3 = ex2(x[e + 3]);
+                sum = add2(sum, a0, a1);
+                sum2 = add2(sum2, a2, a3);
+                pk[c >> 1][(c & 1) * 16 + (e >> 1)] = pack2<T>(a0, a1);
+                pk[c >> 1][(c & 1) * 16 + (e >> 1) + 1] = pack2<T>(a2, a3);
               }
-              if (__builtin_expect(__any_sync(0xffffffffu, row < rows && !(s0 + s1 < kSumLimit)), 0)) {
-                // A score far above the reference (or no number): everything so far is brought to a new one, and these are made again. (O holds the tiles before:
-                // their products were complete before these scores were.)
-                float top = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
-                const float m_new = fmaxf(m_used, m_sub + top), corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
-                const float down = m_sub - (m_new == -INFINITY ? 0.f : m_new);
-                m_used = m_new;
-                l_run *= corr;
-                l0 *= corr;
-                l1 *= corr;
-                tmem_st_wait();
-                tmem_ld_wait();
+            }
+            l0 = lo2(sum) + lo2(sum2);
+            l1 = hi2(sum) + hi2(sum2);
+            done = __all_sync(0xffffffffu, row >= rows || l0 + l1 < kSumLimit);
+            if (done) {
+              tmem_st32(ts, pk[0]);
+              tmem_st32(ts + 32u, pk[1]);
+            }
+          }
+          if (!done) {
+            // 32 scores at a time; their probabilities replace scores that have been read
+            l0 = l1 = 0.f;
+            tmem_ld32_issue(ts, r);
 #pragma unroll 1
-                for (int i = j > 0 ? 0 : D / 16; i < D / 16 + c; ++i) {
-                  const uint32_t at = i < D / 16 ? to + (uint32_t)(i * 16) : ts + (uint32_t)((i - D / 16) * 16);
-                  tmem_ld16_issue(at, pk);
+            for (int c = 0; c < 4; ++c) {
+              uint32_t pk[16];
+              tmem_ld_wait();
+              if (c < live) {  // warp-uniform
+                mask(c);
+                const float m_sub = m_used == -INFINITY ? 0.f : m_used;
+                float x[32];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) fma2(r[e], r[e + 1], p.scale, -m_sub, &x[e], &x[e + 1]);
+                if (c < 3) tmem_ld32_issue(ts + (uint32_t)((c + 1) * 32), r);
+                unsigned long long sum = 0;
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  const float a0 = ex2(x[e]), a1 = ex2(x[e + 1]);
+                  sum = add2(sum, a0, a1);
+                  pk[e >> 1] = pack2<T>(a0, a1);
+                }
+                float s0 = lo2(sum), s1 = hi2(sum);
+                if (__builtin_expect(__any_sync(0xffffffffu, row < rows && !(s0 + s1 < kSumLimit)), 0)) {
+                  // A score far above the reference (or no number): everything so far is brought to a new one, and these are made again. (O holds the tiles before:
+                  // their products were complete before these scores were.)
+                  float top = -INFINITY;
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
+                  const float m_new = fmaxf(m_used, m_sub + top), corr = m_new == -INFINITY ? 1.f : ex2(m_used - m_new);
+                  const float down = m_sub - (m_new == -INFINITY ? 0.f : m_new);
+                  m_used = m_new;
+                  l_run *= corr;
+                  l0 *= corr;
+                  l1 *= corr;
+                  tmem_st_wait();
                   tmem_ld_wait();
+#pragma unroll 1
+                  for (int i = j > 0 ? 0 : D / 16; i < D / 16 + c; ++i) {
+                    const uint32_t at = i < D / 16 ? to + (uint32_t)(i * 16) : ts + (uint32_t)((i - D / 16) * 16);
+                    tmem_ld16_issue(at, pk);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                      const float2 f = unpack2<T>(pk[e]);
+                      pk[e] = i < D / 16 ? __float_as_uint(__uint_as_float(pk[e]) * corr) : pack2<T>(f.x * corr, f.y * corr);
+                    }
+                    tmem_st16(at, pk);
+                  }
+                  tmem_st_wait();
+                  s0 = s1 = 0.f;
 #pragma unroll
                   for (int e = 0; e < 16; ++e) {
-                    const float2 f = unpack2<T>(pk[e]);
-                    pk[e] = i < D / 16 ? __float_as_uint(__uint_as_float(pk[e]) * corr) : pack2<T>(f.x * corr, f.y * corr);
+                    const float a0 = ex2(x[2 * e] + down), a1 = ex2(x[2 * e + 1] + down);
+                    s0 += a0;
+                    s1 += a1;
+                    pk[e] = pack2<T>(a0, a1);
                   }
-                  tmem_st16(at, pk);
                 }
-                tmem_st_wait();
-                s0 = s1 = 0.f;
+                l0 += s0;
+                l1 += s1;
+              } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  const float a0 = ex2(x[2 * e] + down), a1 = ex2(x[2 * e + 1] + down);
-                  s0 += a0;
-                  s1 += a1;
-                  pk[e] = pack2<T>(a0, a1);
-                }
+                for (int e = 0; e < 16; ++e) pk[e] = 0u;
               }
-              l0 += s0;
-              l1 += s1;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) pk[e] = 0u;
+              tmem_st16(ts + (uint32_t)(c * 16), pk);
             }
-            tmem_st16(ts + (uint32_t)(c * 16), pk);
           }
           l_run += l0 + l1;
           tmem_st_wait();
