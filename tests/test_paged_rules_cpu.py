@@ -11,7 +11,7 @@ CSRC = os.path.join(ROOT, "turbotransformers_b200", "csrc")
 
 
 class Split(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int) for n in ("block_heads", "blocks", "head_blocks", "tile_tokens", "unit", "causal")]
+    _fields_ = [(n, ctypes.c_int) for n in ("block_heads", "blocks", "head_blocks", "tile_tokens", "unit_shift", "causal")]
 
 
 class Place(ctypes.Structure):

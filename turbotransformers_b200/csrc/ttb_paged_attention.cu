@@ -21,8 +21,9 @@ using namespace ttb::sm100;
 namespace {
 
 constexpr int kWarps = 4, kLoaders = 4, kThreads = (kWarps + kLoaders) * 32;
-constexpr int kRows = kFewRows;
-constexpr int kBlock = 32;  // a warp's keys of a unit
+constexpr int kBlock = 32;             // a warp's keys of a unit
+constexpr int kParts = 4;              // worked out ahead
+constexpr float kSumLimit = 32768.0f;  // a sum of probabilities below this keeps each of them inside fp16's and bf16's range
 static_assert(kBlock * kWarps == kUnit, "the four warps share a unit");
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -43,53 +44,60 @@ template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int D> struct Shape {
+// A tile of NT groups of eight query rows.
+template <int D, int NT> struct Shape {
+  static constexpr int kRows = 8 * NT;
   static constexpr int kHalves = D / 64;
   static constexpr int kHalfBytes = kUnit * 128;
   static constexpr int kTile = kHalves * kHalfBytes;  // 128 keys, or 128 values
   static constexpr int kStages = D == 128 ? 3 : 6;
   static constexpr int kQHalf = kRows * 128;
-  static constexpr int kQ = kStages * 2 * kTile;       // two tiles' queries
-  static constexpr int kJoin = kQ + 2 * kHalves * kQHalf;  // float [2][kRows][D]
-  static constexpr int kPrefix = kJoin + 2 * kRows * D * 4;
-  static constexpr int kScratch = kPrefix + (kMaxSequences + 1) * 8;
-  static constexpr int kStats = kScratch + kThreads / 32 * 8;
-  static constexpr int kBars = kStats + kWarps * kRows * 8;
-  static constexpr int kNumBars = 2 * kStages + 4;
+  static constexpr int kQ = kStages * 2 * kTile;
+  static constexpr int kPitch = D + 4;                       // floats between rows of the states that are joined (no bank conflicts)
+  static constexpr int kJoin = kQ + 2 * kHalves * kQHalf;  // float [kWarps][8][kPitch]; before the first part, the sequences' places
+  static constexpr int kStats = kJoin + kWarps * 8 * kPitch * 4;   // float2 [2][kWarps][kRows]
+  static constexpr int kScratch = kStats + 2 * kWarps * kRows * 8;
+  static constexpr int kWorks = kScratch + kThreads / 32 * 8;
+  static constexpr int kBars = kWorks + kParts * (int)sizeof(Work);
+  static constexpr int kNumBars = 2 * kStages + 5 + 2 * kParts;
   static constexpr int kBytes = kBars + kNumBars * 8 + 16;
+  static_assert(kWarps * 8 * kPitch * 4 >= (kMaxSequences + 1) * 8, "the sequences' places");
 };
 
-__device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // of the four computing warps
-__device__ __forceinline__ bool warps_all(bool mine) {
-  int all;
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      "setp.ne.b32 p, %1, 0;\n"
-      "bar.red.and.pred q, 1, 128, p;\n"
-      "selp.u32 %0, 1, 0, q;\n"
-      "}\n"
-      : "=r"(all)
-      : "r"((int)mine)
-      : "memory");
-  return all != 0;
+// An 8 x 8 matrix of 16-bit pairs, transposed across the warp.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float column_max(float v) {  // over the lanes that hold the same column
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params p) {
-  using S = Shape<D>;
+  using S = Shape<D, NT>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  long long* prefix = reinterpret_cast<long long*>(smem + S::kPrefix);
   float* join = reinterpret_cast<float*>(smem + S::kJoin);
-  float2* stats = reinterpret_cast<float2*>(smem + S::kStats);  // [kWarps][kRows]
+  float2* stats = reinterpret_cast<float2*>(smem + S::kStats);
+  Work* works = reinterpret_cast<Work*>(smem + S::kWorks);
   const uint32_t bar0 = smem_u32(smem + S::kBars);
-  auto full = [&](uint32_t g) { return bar0 + 8 * (g % S::kStages); };
-  auto empty = [&](uint32_t g) { return bar0 + 8 * (S::kStages + g % S::kStages); };
+  auto bar = [&](int k) { return bar0 + 8u * k; };
+  auto full = [&](uint32_t g) { return bar((int)(g % S::kStages)); };
+  auto empty = [&](uint32_t g) { return bar(S::kStages + (int)(g % S::kStages)); };
   auto phase = [&](uint32_t g) { return (g / S::kStages) & 1u; };
-  auto q_full = [&](uint32_t n) { return bar0 + 8 * (2 * S::kStages + (n & 1)); };
-  auto q_empty = [&](uint32_t n) { return bar0 + 8 * (2 * S::kStages + 2 + (n & 1)); };
+  auto q_full = [&](uint32_t n) { return bar(2 * S::kStages + (int)(n & 1)); };
+  auto q_empty = [&](uint32_t n) { return bar(2 * S::kStages + 2 + (int)(n & 1)); };
+  auto q_phase = [&](uint32_t n) { return (n >> 1) & 1u; };
+  auto q_at = [&](uint32_t n) { return base + S::kQ + (n & 1) * S::kHalves * S::kQHalf; };
+  auto part_full = [&](uint32_t n) { return bar(2 * S::kStages + 5 + (int)(n % kParts)); };
+  auto part_empty = [&](uint32_t n) { return bar(2 * S::kStages + 5 + kParts + (int)(n % kParts)); };
+  auto part_phase = [&](uint32_t n) { return (n / kParts) & 1u; };
+  const uint32_t meet = bar(2 * S::kStages + 4);  // the computing warps'
   auto keys_at = [&](uint32_t g) { return base + (g % S::kStages) * 2 * S::kTile; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kBars + S::kNumBars * 8);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -101,9 +109,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(empty(i), kWarps);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full(i), 1);
-      mbar_init(q_empty(i), kWarps);
+      mbar_init(bar(2 * S::kStages + i), 1);
+      mbar_init(bar(2 * S::kStages + 2 + i), kWarps);
     }
+    for (int i = 0; i < kParts; ++i) {
+      mbar_init(part_full(i), 1);
+      mbar_init(part_empty(i), kWarps + kLoaders - 1);
+    }
+    mbar_init(meet, kWarps);
     *abort_flag = 0;
     prefetch_tensormap(&tm_q);
     prefetch_tensormap(&tm_k);
@@ -111,63 +124,91 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     mbar_init_fence();
   }
   pdl_wait();
+  long long* prefix = reinterpret_cast<long long*>(smem + S::kJoin);
   const long long total = line_up(p, prefix, reinterpret_cast<long long*>(smem + S::kScratch), kThreads);
   const int ctas = ctas_of(total, (int)gridDim.x, 1), cta = blockIdx.x;
   if (cta >= ctas) {
     if (tid == 0) p.parts.cuts[cta].pieces = 0;
     return;
   }
-  const long long lo = first_unit(total, ctas, cta), hi = first_unit(total, ctas, cta + 1);
-  Part t = part_at(p, prefix, lo, hi - lo);
+  // The n-th part, for every warp but the one that works them out. False: no part, there are no more or something gave up.
+  auto take_part = [&](uint32_t n, Work* w) {
+    if (!__all_sync(0xffffffffu, mbar_wait(part_full(n), part_phase(n), abort_flag))) return false;
+    *w = works[n % kParts];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(part_empty(n));
+    return w->units >= 0;
+  };
 
   if (warp >= kWarps) {
     // ---- loads: a lane for each box (a page, or 128 keys) of keys or values and half of a head, every fourth of them a warp's: a copy takes its thread some 60
-    // cycles to issue, one lane after the other. The pages of a unit are looked up while the one before is loaded.
+    // cycles to issue, one lane after the other. The pages of a unit are looked up while the one before is loaded. The first of the warps works the parts out.
     const int loader = warp - kWarps;
     const int page_tokens = 1 << p.s.page_shift, box_rows = min(page_tokens, kUnit);
     const int at = lane * kLoaders + loader, box = at / (2 * S::kHalves), which = at / S::kHalves & 1, half = at % S::kHalves;
+    const long long lo = first_unit(total, ctas, cta), hi = first_unit(total, ctas, cta + 1);
     uint32_t g = 0, n = 0;
-    bool ok = true;
-    auto page_at = [&](const Part& t, int key0) {
-      const int key = key0 + box * box_rows;
-      if (key >= t.keys || box * box_rows >= kUnit) return -1;
-      bool bad;
-      const int page = page_of(p.s, t.b, key, &bad);
-      if (bad) bad_index(p.s.status);
-      return bad ? 0 : page;
+    bool ok = true, cut_here = false;
+    long long u = lo;
+    Part t = {};
+    auto publish = [&](Work* w) {
+      w->units = -1;
+      if (n > 0) u += t.take;
+      if (u < hi) {
+        if (n > 0) next_part(p, t, hi - u);
+        else t = part_at(p, prefix, lo, hi - lo);
+        *w = work_of(p, t, 2 * cta + (u == lo ? 0 : 1));
+        if (w->slot >= 0 && t.first == 0) {
+          cut_here = true;
+          if (lane == 0) p.parts.cuts[cta] = cut_of(p, t, u, total, cta, ctas, w->slot);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(part_empty(n), part_phase(n) ^ 1u, abort_flag));
+      if (ok && lane == 0) works[n % kParts] = *w;
+      __syncwarp();
+      if (ok && lane == 0) mbar_arrive(part_full(n));
+      return ok && w->units >= 0;
     };
-    int page = page_at(t, (int)t.first * kUnit);
-    for (long long u = lo; u < hi && ok;) {
-      const int k_end = min((int)(t.first + t.take) * kUnit, t.keys), y0 = t.block / p.split.head_blocks << p.s.page_shift;
-      if (loader == 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(q_empty(n), (n >> 1 & 1u) ^ 1u, abort_flag));
-        if (!ok) break;
+    auto page_at = [&](const Work& w, int i) {  // (looked at when it is needed)
+      const int key = (w.first + i) * kUnit + box * box_rows;
+      return key < w.keys && box * box_rows < kUnit ? p.s.table[w.b * p.s.table_stride + (key >> p.s.page_shift)] : 0;
+    };
+    Work w = {}, w2;
+    int page = 0;
+    for (;; ++n) {  // w2 is the n-th part; the loads are those of w, the one before
+      const bool more = loader == 0 ? publish(&w2) : take_part(n, &w2);
+      if (w.units == 0 && more) page = page_at(w2, 0);  // at the beginning, and behind a part without keys (more tokens than the table lists)
+      if (n > 0 && loader == 0 && ok) {
+        ok = __all_sync(0xffffffffu, mbar_wait(q_empty(n - 1), q_phase(n - 1) ^ 1u, abort_flag));
+        if (ok && lane == 0) {
+          mbar_expect_tx(q_full(n - 1), (uint32_t)(p.split.tile_tokens * p.split.block_heads * D * 2));
+          for (int h = 0; h < S::kHalves; ++h) tma_load_3d(q_at(n - 1) + h * S::kQHalf, &tm_q, q_full(n - 1), h * 64, w.head0, w.tok0);
+        }
       }
-      if (loader == 0 && lane == 0) {
-        mbar_expect_tx(q_full(n), (uint32_t)(p.split.tile_tokens * p.split.block_heads * D * 2));
-        for (int h = 0; h < S::kHalves; ++h)
-          tma_load_3d(base + S::kQ + (n & 1) * S::kHalves * S::kQHalf + h * S::kQHalf, &tm_q, q_full(n), h * 64, first_head(p, t.block), t.tok0);
-      }
-      ++n;
-      const long long next = u + t.take;
-      Part t2 = t;
-      if (next < hi) next_part(p, t2, hi - next);
-      if ((int)t.first * kUnit >= k_end && next < hi) page = page_at(t2, (int)t2.first * kUnit);  // a part without keys (more tokens than the table lists)
-      for (int k0 = (int)t.first * kUnit; k0 < k_end; k0 += kUnit, ++g) {
-        const int mine = page;
-        page = k0 + kUnit < k_end ? page_at(t, k0 + kUnit) : next < hi ? page_at(t2, (int)t2.first * kUnit) : -1;
+      for (int i = 0; i < w.units && ok; ++i, ++g) {
+        const int key = (w.first + i) * kUnit + box * box_rows;
+        int mine = -1;
+        if (key < w.keys && box * box_rows < kUnit) {
+          mine = page;
+          if (mine < 0 || mine >= p.s.pages) {
+            bad_index(p.s.status);
+            mine = 0;
+          }
+        }
+        page = i + 1 < w.units ? page_at(w, i + 1) : more ? page_at(w2, 0) : 0;
         ok = __all_sync(0xffffffffu, mbar_wait(empty(g), phase(g) ^ 1u, abort_flag));
         if (!ok) break;
-        const int mine_boxes = __popc(__ballot_sync(0xffffffffu, mine >= 0));
-        if (lane == 0) mbar_expect_tx(full(g), (uint32_t)(mine_boxes * box_rows * 128));
+        const int boxes = __popc(__ballot_sync(0xffffffffu, mine >= 0));
+        if (lane == 0) mbar_expect_tx(full(g), (uint32_t)(boxes * box_rows * 128));
         __syncwarp();
         if (mine >= 0)
           tma_load_3d(keys_at(g) + which * S::kTile + half * S::kHalfBytes + box * box_rows * 128, which ? &tm_v : &tm_k, full(g), half * 64,
-                      y0 + ((k0 + box * box_rows) & (page_tokens - 1)), mine);
+                      w.key_row + (key & (page_tokens - 1)), mine);
       }
-      t = t2;
-      u = next;
+      if (!more || !ok) break;
+      w = w2;
     }
+    if (loader == 0 && !cut_here && lane == 0) p.parts.cuts[cta].pieces = 0;
     if (*abort_flag) {  // copies in flight land before shared memory is given back
       const long long t0 = clock64();
       while (clock64() - t0 < 4000000LL) {
@@ -176,191 +217,235 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     return;
   }
 
-  // ---- computation: warp w takes keys 32 w to 32 w + 31 of every unit
-  bool cut_here = false, ok = true;
-  uint32_t g = 0, n = 0;
-  for (long long u = lo; u < hi; ++n) {
-    const int head0 = first_head(p, t.block), heads = heads_of(p, t.block);
-    int limit[2];  // keys that rows lane / 4 and lane / 4 + 8 see
+  // ---- computation: warp w takes keys 32 w to 32 w + 31 of every unit. Keys are the rows of the products and queries their columns, so that a tile of eight query rows
+  // leaves none of the product empty: S^T = K Q^T, O^T = V^T P^T, with the probabilities transposed in between.
+  bool ok = true;
+  uint32_t g = 0, n_meet = 0;
+  // A barrier of the four warps that gives up like every wait.
+  auto together = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(meet);
+    ok = __all_sync(0xffffffffu, mbar_wait(meet, n_meet++ & 1u, abort_flag));
+    return ok;
+  };
+  Work t;
+  for (uint32_t n = 0; take_part(n, &t); ++n) {
+    constexpr bool kQInRegisters = NT <= 2;
+    uint32_t qf[kQInRegisters ? D / 32 : 1][NT][4];
+    auto load_q = [&](int j, uint32_t (&q)[4], int nt) {  // columns 32 j to 32 j + 31 of eight queries: two products' operands
+      const int row = nt * 8 + (lane & 7), c = (j & 1) * 4 + (lane >> 3);
+      ldsm_x4(q, q_at(n) + (j >> 1) * S::kQHalf + row * 128 + ((c ^ (row & 7)) << 4));
+    };
+    ok = __all_sync(0xffffffffu, mbar_wait(q_full(n), q_phase(n), abort_flag));
+    if (!ok) break;
+    if constexpr (kQInRegisters) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = (lane >> 2) + r * 8;
-      limit[r] = p.split.causal && row < t.rows ? min(t.pos0 + row / p.split.block_heads + 1, t.keys) : t.keys;
-    }
-    uint32_t qf[D / 16][4];
-    ok = ok && mbar_wait(q_full(n), n >> 1 & 1u, abort_flag);
-    if (ok) {
-      const uint32_t q = base + S::kQ + (n & 1) * S::kHalves * S::kQHalf;
+      for (int j = 0; j < D / 32; ++j)
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int row = lane & 15, c = (k & 3) * 2 + (lane >> 4);
-        ldsm_x4(qf[k], q + (k >> 2) * S::kQHalf + row * 128 + ((c ^ (row & 7)) << 4));
-      }
+        for (int nt = 0; nt < NT; ++nt) load_q(j, qf[j][nt], nt);
       __syncwarp();
       if (lane == 0) mbar_arrive(q_empty(n));
     }
     const int all_see = p.split.causal ? min(t.pos0 + 1, t.keys) : t.keys;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
+    // this lane's queries are columns 2 (lane % 4) and the next of every group: their reference, the sums of its keys, and of their outputs rows lane / 4 and + 8
+    float m[NT][2], l[NT][2], o[D / 16][NT][4];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-
-    const int k_end = min((int)(t.first + t.take) * kUnit, t.keys);
-    for (int u0 = (int)t.first * kUnit; u0 < k_end && ok; u0 += kUnit, ++g) {
-      ok = mbar_wait(full(g), phase(g), abort_flag);
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][nt][e] = 0.f;
+    }
+    bool fresh = true;
+    for (int i = 0; i < t.units; ++i, ++g) {
+      ok = __all_sync(0xffffffffu, mbar_wait(full(g), phase(g), abort_flag));
       if (!ok) break;
-      const int k0 = u0 + warp * kBlock;
+      const int k0 = (t.first + i) * kUnit + warp * kBlock;
       if (k0 < t.keys) {
         const uint32_t kt = keys_at(g) + warp * kBlock * 128, vt = kt + S::kTile;
         if (k0 + kBlock > t.keys) {
           // rows behind the last key: what the page or the ring happens to hold there, which a probability of zero does not undo where it is not finite
-          for (int i = lane; i < (kBlock - (t.keys - k0)) * S::kHalves * 8; i += 32) {
-            const int r = (t.keys - k0) + i / (S::kHalves * 8), c = i % (S::kHalves * 8);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (c >> 3) * S::kHalfBytes + r * 128 + (c & 7) * 16), "r"(0) : "memory");
+#pragma unroll 1
+          for (int c = lane; c < (kBlock - (t.keys - k0)) * S::kHalves * 8; c += 32) {
+            const int r = (t.keys - k0) + c / (S::kHalves * 8), col = c % (S::kHalves * 8);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + (col >> 3) * S::kHalfBytes + r * 128 + (col & 7) * 16), "r"(0) : "memory");
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next load into these rows
           __syncwarp();
         }
-        float s[4][4];
+        float s[2][NT][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
+            for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
 #pragma unroll
-          for (int n2 = 0; n2 < 2; ++n2) {  // 16 keys: matrices (keys 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-            const int row = n2 * 16 + (lane & 7) + ((lane >> 4) << 3), c = (k & 3) * 2 + ((lane >> 3) & 1);
-            uint32_t b[4];
-            ldsm_x4(b, kt + (k >> 2) * S::kHalfBytes + row * 128 + ((c ^ (row & 7)) << 4));
-            mma16816<T>(s[n2 * 2], qf[k], b[0], b[1]);
-            mma16816<T>(s[n2 * 2 + 1], qf[k], b[2], b[3]);
+        for (int j = 0; j < D / 32; ++j) {
+          if constexpr (!kQInRegisters) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) load_q(j, qf[0][nt], nt);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {  // 16 keys x 16 columns
+              const int row = mt * 16 + (lane & 15), c = (j & 1) * 4 + k * 2 + (lane >> 4);
+              uint32_t a[4];
+              ldsm_x4(a, kt + (j >> 1) * S::kHalfBytes + row * 128 + ((c ^ (row & 7)) << 4));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const uint32_t (&q)[4] = qf[kQInRegisters ? j : 0][nt];
+                mma16816<T>(s[mt][nt], a, q[2 * k], q[2 * k + 1]);
+              }
+            }
           }
         }
         if (k0 + kBlock > all_see) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (k0 + i * 8 + (lane & 3) * 2 + (e & 1) >= limit[e >> 1]) s[i][e] = -INFINITY;
-        }
-        uint32_t pf[2][4];
+            for (int q = 0; q < 2; ++q) {
+              const int row = nt * 8 + (lane & 3) * 2 + q;
+              const int limit = (p.split.causal && row < t.rows ? min(t.pos0 + row / p.split.block_heads + 1, t.keys) : t.keys) - k0 - (lane >> 2);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(s[i][2 * r], s[i][2 * r + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float m_new = fmaxf(m[r], mx * p.scale), sub = m_new == -INFINITY ? 0.f : m_new;
-          const float corr = ex2(m[r] - sub);
-          m[r] = m_new;
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = ex2(fmaf(s[i][2 * r], p.scale, -sub)), b = ex2(fmaf(s[i][2 * r + 1], p.scale, -sub));
-            sum += a + b;
-            pf[i >> 1][(i & 1) * 2 + r] = pack2<T>(a, b);
-          }
-          l[r] = l[r] * corr + sum;  // of this lane's columns
-          if (__any_sync(0xffffffffu, corr != 1.f)) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-              o[i][2 * r] *= corr;
-              o[i][2 * r + 1] *= corr;
+              for (int x = 0; x < 4; ++x)
+                if (x * 8 >= limit) s[x >> 1][nt][(x & 1) * 2 + q] = -INFINITY;
             }
+        }
+        // A row's reference is the maximum of its first keys; it is raised (and the sums rescaled) only where probabilities sum up to 2^15 and more: the division by
+        // the sum makes the result independent of it.
+        uint32_t pf[2][NT][2];
+        while (true) {
+          if (fresh) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const float top = column_max(fmaxf(fmaxf(s[0][nt][q], s[0][nt][2 + q]), fmaxf(s[1][nt][q], s[1][nt][2 + q]))) * p.scale;
+                const float m_new = fmaxf(m[nt][q], top), corr = m_new == -INFINITY ? 1.f : ex2(m[nt][q] - m_new);
+                m[nt][q] = m_new;
+                l[nt][q] *= corr;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                  o[d][nt][q] *= corr;
+                  o[d][nt][2 + q] *= corr;
+                }
+              }
+          }
+          bool far = false;
+          float sum[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+            sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const float a = ex2(fmaf(s[mt][nt][2 * r], p.scale, -m0)), b = ex2(fmaf(s[mt][nt][2 * r + 1], p.scale, -m1));
+                sum[nt][0] += a;
+                sum[nt][1] += b;
+                pf[mt][nt][r] = pack2<T>(a, b);
+              }
+            const int row = nt * 8 + (lane & 3) * 2;
+            far = far || (row < t.rows && !(sum[nt][0] < kSumLimit)) || (row + 1 < t.rows && !(sum[nt][1] < kSumLimit));
+          }
+          if (fresh || !__any_sync(0xffffffffu, far)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              l[nt][0] += sum[nt][0];
+              l[nt][1] += sum[nt][1];
+            }
+            break;
+          }
+          fresh = true;
+        }
+        fresh = false;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) pf[mt][nt][r] = transposed(pf[mt][nt][r]);
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {  // 16 columns of the values x 16 keys
+            const int row = mt * 16 + (lane & 7) + ((lane >> 4) << 3), c = (d & 3) * 2 + ((lane >> 3) & 1);
+            uint32_t a[4];
+            ldsm_x4_trans(a, vt + (d >> 2) * S::kHalfBytes + row * 128 + ((c ^ (row & 7)) << 4));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[d][nt], a, pf[mt][nt][0], pf[mt][nt][1]);
           }
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int n2 = 0; n2 < D / 16; ++n2) {  // 16 keys x 16 columns of the values
-            const int row = k * 16 + (lane & 15), c = (n2 & 3) * 2 + (lane >> 4);
-            uint32_t b[4];
-            ldsm_x4_trans(b, vt + (n2 >> 2) * S::kHalfBytes + row * 128 + ((c ^ (row & 7)) << 4));
-            mma16816<T>(o[n2 * 2], pf[k], b[0], b[1]);
-            mma16816<T>(o[n2 * 2 + 1], pf[k], b[2], b[3]);
-          }
         __syncwarp();
       }
       if (lane == 0) mbar_arrive(empty(g));
     }
-    // ---- the four warps' states become one
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if ((lane & 3) == 0) stats[warp * kRows + (lane >> 2) + r * 8] = make_float2(m[r], l[r]);
+    if constexpr (!kQInRegisters) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_empty(n));
     }
-    if (!warps_all(ok)) { ok = false; break; }
-    float M[2], L[2], w[2];
+    // ---- the four warps' states become one, eight rows at a time
+    float2* mine = stats + (n & 1) * kWarps * S::kRows;  // (the part before's may still be read)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = (lane >> 2) + r * 8;
-      M[r] = -INFINITY;
-      for (int i = 0; i < kWarps; ++i) M[r] = fmaxf(M[r], stats[i * kRows + row].x);
-      const float sub = M[r] == -INFINITY ? 0.f : M[r];
-      L[r] = 0.f;
-      for (int i = 0; i < kWarps; ++i) L[r] += stats[i * kRows + row].y * ex2(stats[i * kRows + row].x - sub);
-      w[r] = ex2(m[r] - sub);
-    }
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+      for (int q = 0; q < 2; ++q) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] *= w[e >> 1];
-#pragma unroll
-    for (int half = 2; half > 0; half >>= 1) {  // warps 2, 3 to 0, 1; then 1 to 0
-      float* mine = join + (warp & (half - 1)) * kRows * D;
-      if (warp >= half && warp < 2 * half) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-            *reinterpret_cast<float2*>(mine + ((lane >> 2) + r * 8) * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+        for (int x = 4; x < 32; x <<= 1) l[nt][q] += __shfl_xor_sync(0xffffffffu, l[nt][q], x);
+        if (lane < 4) mine[warp * S::kRows + nt * 8 + lane * 2 + q] = make_float2(m[nt][q], l[nt][q]);
       }
-      warps_sync();
-      if (warp < half) {
+    if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
+    for (int nt = 0; nt < NT; ++nt) {
+      if (nt * 8 >= t.rows) break;
+      if (!together()) break;  // the rows before have been read
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float2 v = *reinterpret_cast<const float2*>(mine + ((lane >> 2) + r * 8) * D + i * 8 + (lane & 3) * 2);
-            o[i][2 * r] += v.x;
-            o[i][2 * r + 1] += v.y;
-          }
-      }
-      warps_sync();
-    }
-    const bool whole = t.take == t.units;
-    const int slot = 2 * cta + (u == lo ? 0 : 1);
-    if (warp == 0) {
+      for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = (lane >> 2) + r * 8, i = row / p.split.block_heads, h = row % p.split.block_heads;
-        if (row >= t.rows || h >= heads) continue;
-        if (whole) {
-          const float inv = L[r] == 0.f ? 0.f : 1.f / L[r];
-          T* dst = static_cast<T*>(p.out) + (long long)(t.tok0 + i) * p.ldo + (long long)(head0 + h) * D + (lane & 3) * 2;
+        for (int e = 0; e < 4; ++e) {
+          const int q = (lane & 3) * 2 + (e & 1);
+          if (nt * 8 + q < t.rows) join[(warp * 8 + q) * S::kPitch + d * 16 + (lane >> 2) + (e >> 1) * 8] = o[d][nt][e];
+        }
+      if (!together()) break;
+      const int tasks = min(8, t.rows - nt * 8) * (D / 4);
+      for (int x = tid; x < tasks; x += kWarps * 32) {
+        const int q = x / (D / 4), d = x % (D / 4) * 4, row = nt * 8 + q, i = row / p.split.block_heads, h = row % p.split.block_heads;
+        if (h >= t.heads) continue;
+        float M = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint32_t*>(dst + c * 8) = pack2<T>(o[c][2 * r] * inv, o[c][2 * r + 1] * inv);
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mine[w * S::kRows + row].x);
+        const float sub = M == -INFINITY ? 0.f : M;
+        float L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = mine[w * S::kRows + row];
+          const float f = ex2(ml.x - sub);
+          const float4 a = *reinterpret_cast<const float4*>(join + (w * 8 + q) * S::kPitch + d);
+          L = fmaf(ml.y, f, L);
+          v[0] = fmaf(a.x, f, v[0]);
+          v[1] = fmaf(a.y, f, v[1]);
+          v[2] = fmaf(a.z, f, v[2]);
+          v[3] = fmaf(a.w, f, v[3]);
+        }
+        if (t.slot < 0) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          uint2 y;
+          y.x = pack2<T>(v[0] * inv, v[1] * inv);
+          y.y = pack2<T>(v[2] * inv, v[3] * inv);
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (long long)(t.tok0 + i) * p.ldo + (long long)(t.head0 + h) * D + d) = y;
         } else {
-          float* dst = p.parts.o + ((long long)slot * kRows + row) * D + (lane & 3) * 2;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) *reinterpret_cast<float2*>(dst + c * 8) = make_float2(o[c][2 * r], o[c][2 * r + 1]);
-          if ((lane & 3) == 0) p.parts.ml[(long long)slot * kRows + row] = make_float2(M[r], L[r]);
+          const long long to = (long long)t.slot * S::kRows + row;
+          *reinterpret_cast<float4*>(p.parts.o + to * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+          if (d == 0) p.parts.ml[to] = make_float2(M, L);
         }
       }
     }
-    if (!whole && t.first == 0) {  // the tile's beginning is here, its rest the next CTAs'
-      cut_here = true;
-      if (tid == 0) p.parts.cuts[cta] = cut_of(p, t, u, total, cta, ctas, slot);
-    }
-    u += t.take;
-    if (u < hi) next_part(p, t, hi - u);
+    if (!ok) break;
   }
-  if (!cut_here && tid == 0) p.parts.cuts[cta].pieces = 0;
-  if (!ok && lane == 0) atomicExch(p.s.status, (int)TTB_ERR_DEVICE_WAIT);
+  if ((!ok || *abort_flag) && lane == 0) atomicExch(p.s.status, (int)TTB_ERR_DEVICE_WAIT);
 }
 
 // Joins the parts of the tiles that were cut, of both kernels: a block (and its neighbours along y) for each of their CTAs, a warp for each row, parts in the
@@ -405,11 +490,14 @@ paged_join_kernel(const JoinParams p) {
         float x[8][V];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
+          if (k1 + e < n) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) x[e][v] = parts.o[at(min(k0 + k1 + e, c.pieces - 1)) * D + v * 32 + lane];
+            for (int v = 0; v < V; ++v) x[e][v] = parts.o[at(k0 + k1 + e) * D + v * 32 + lane];
+          }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float w = __shfl_sync(0xffffffffu, mine, k1 + e);  // zero behind the last, and for a part without a key for this row, which has no sums
+          if (k1 + e >= n) break;
+          const float w = __shfl_sync(0xffffffffu, mine, k1 + e);  // zero for a part without a key for this row, which has no sums
 #pragma unroll
           for (int v = 0; v < V; ++v) o[v] = w == 0.f ? o[v] : fmaf(x[e][v], w, o[v]);
         }
@@ -423,31 +511,34 @@ paged_join_kernel(const JoinParams p) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 int launch_rows(ttb_ctx* ctx, const ttb_paged_kv* kv, int64_t heads, const Params& p) {
-  using S = Shape<D>;
+  using S = Shape<D, NT>;
   CUtensorMap tm_q, tm_k, tm_v;
   if (!encode_maps(kv, std::is_same<T, __nv_bfloat16>::value, heads, p, p.split.tile_tokens, &tm_q, &tm_k, &tm_v))
     return fail(ctx, TTB_ERR_CUDA, "paged_attention: a tensor map was refused");
   static bool configured[64] = {};
   const int dev = ctx->device < 64 ? ctx->device : 63;
   if (!configured[dev]) {
-    TTB_CUDA(ctx, cudaFuncSetAttribute(paged_rows_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    TTB_CUDA(ctx, cudaFuncSetAttribute(paged_rows_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     configured[dev] = true;
   }
-  launch_pdl(paged_rows_kernel<T, D>, dim3((unsigned)ctx->sm_count), dim3(kThreads), S::kBytes, ctx->stream, tm_q, tm_k, tm_v, p);
+  launch_pdl(paged_rows_kernel<T, D, NT>, dim3((unsigned)ctx->sm_count), dim3(kThreads), S::kBytes, ctx->stream, tm_q, tm_k, tm_v, p);
   return launched(ctx, "paged_attention");
 }
 
 template <typename T, int D>
 int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, Params& p) {
-  // Which kernel: sequences whose new tokens make kFewRows rows at most go to the one for few rows, the others to the other. The host knows the lengths'
-  // sum only: with no more tokens than sequences one kernel takes all, whatever a single sequence has.
-  const int few = p.group <= kFewRows ? kFewRows / p.group : 0;
-  const bool one = kv->B == 1, rows_only = few > 0 && p.s.tokens <= (one ? few : (int)kv->B), many_only = few == 0 || (one && !rows_only);
+  // Which kernels, and the rows of a tile of the one for few. The host knows the sum of the new tokens only. With no more tokens than sequences, tiles of a token's rows (up to 32)
+  // take all of them, a sequence of several tokens several tiles. Otherwise tiles of an average sequence's rows, 16 at most, and the sequences that have more go
+  // to the kernel for many (16 requests of 3 to 6 tokens, 8 heads to a key head, over up to 16000: 143 us there, 171 with those of 32 rows in this one).
+  const int64_t tokens = p.s.tokens, B = kv->B, each = (tokens + B - 1) / B * p.group;
+  const int64_t need = std::max<int64_t>(p.group, std::min<int64_t>(each, 16));
+  const int groups = need <= 8 ? 1 : need <= 16 ? 2 : 4, few = 8 * groups / p.group;
+  const bool rows_only = few > 0 && tokens <= (B == 1 ? few : B), many_only = few == 0 || (B == 1 && !rows_only);
   const int ctas = ctx->sm_count;
   size_t at = 0, o[2], ml[2], cuts[2];
-  const int rows[2] = {kFewRows, kManyRows};
+  const int rows[2] = {8 * groups, kManyRows};
   const bool used[2] = {!many_only, !rows_only};
   auto take = [&](size_t bytes) { const size_t x = at; at = (at + bytes + 255) & ~(size_t)255; return x; };
   for (int i = 0; i < 2; ++i) {
@@ -472,15 +563,15 @@ int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, P
     j.parts[n] = p.parts;
     j.rows[n++] = rows[i];
     if (i == 0) {
-      p.split = split_of((int)heads, (int)kv->kv_heads, kFewRows, 1, kUnit, p.split.causal);
-      st = launch_rows<T, D>(ctx, kv, heads, p);
+      p.split = split_of((int)heads, (int)kv->kv_heads, rows[0], 1, kUnit, p.split.causal);
+      st = groups == 1 ? launch_rows<T, D, 1>(ctx, kv, heads, p) : groups == 2 ? launch_rows<T, D, 2>(ctx, kv, heads, p) : launch_rows<T, D, 4>(ctx, kv, heads, p);
     } else {
       p.split = split_of((int)heads, (int)kv->kv_heads, kManyRows / 2, 2, kUnit, p.split.causal);
       st = paged_tc_launch(ctx, dtype, kv, heads, p);
     }
   }
   if (!st) {
-    launch_pdl(paged_join_kernel<T, D>, dim3((unsigned)ctas, used[1] ? 16 : kFewRows / 4, (unsigned)n), dim3(128), 0, ctx->stream, j);
+    launch_pdl(paged_join_kernel<T, D>, dim3((unsigned)ctas, used[1] ? 16 : rows[0] / 4, (unsigned)n), dim3(128), 0, ctx->stream, j);
     st = launched(ctx, "paged_attention_join");
   }
   const int f = ttb_free(ctx, ws, "paged_attention/parts");

@@ -11,8 +11,7 @@ namespace paged {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kUnit = 128;    // keys
-constexpr int kFewRows = 16;  // of a tile of the kernel for few rows
-constexpr int kManyRows = 256;
+constexpr int kManyRows = 256;  // of a tile of the kernel for many rows
 
 // A tile that was cut, written by the CTA that has its beginning.
 struct Cut {
@@ -171,6 +170,39 @@ __device__ __forceinline__ Cut cut_of(const Params& p, const Part& t, long long 
 #pragma unroll 1
   while (cta + pieces < ctas && first_unit(total, ctas, cta + pieces) < u + t.units) ++pieces;
   return Cut{pieces, slot, t.tok0, first_head(p, t.block), t.rows, p.split.block_heads, heads_of(p, t.block)};
+}
+
+// A part of the line as a CTA's warps read it: one of them works it out, the others would have its code in the instruction cache besides (with it in every role the kernel
+// for many rows was 192 KB long, and the products stood still for instructions).
+struct Work {
+  int units;       // that have keys; -1: there is no more
+  int turns;       // many rows: both sets hold the same rows and take the units in turn
+  int count[2];    // and each set's units
+  int first;       // the part's first unit in its tile
+  int b, key_row;  // sequence, and the key head's first row in a page
+  int keys, pos0, tok0, rows;  // as in Part
+  int head0, heads;
+  int slot;        // of its sums, -1: the tile is whole
+  int pad[2];
+};
+constexpr int kRingWorks = 8;
+
+__device__ __forceinline__ Work work_of(const Params& p, const Part& t, int slot) {
+  Work w;
+  w.units = max(0, min(t.take, (t.keys + kUnit - 1) / kUnit - (int)t.first));
+  w.turns = w.count[0] = w.count[1] = 0;
+  w.first = (int)t.first;
+  w.b = t.b;
+  w.key_row = t.block / p.split.head_blocks << p.s.page_shift;
+  w.keys = t.keys;
+  w.pos0 = t.pos0;
+  w.tok0 = t.tok0;
+  w.rows = t.rows;
+  w.head0 = first_head(p, t.block);
+  w.heads = heads_of(p, t.block);
+  w.slot = t.take == t.units ? -1 : slot;
+  w.pad[0] = w.pad[1] = 0;
+  return w;
 }
 
 // The tensor maps: boxes of `tokens` tokens of a head block's queries, of a page (128 tokens at most) of one key head's keys and values; 64 elements wide each.

@@ -30,21 +30,6 @@ constexpr uint32_t kTmemCols = 512;
 constexpr float kSumLimit = 32768.0f;  // a sum of probabilities below this keeps each of them inside fp16's and bf16's range
 static_assert(kUnit == 128 && kSet == 128, "the products are 128 x 128");
 
-// A part of the line as the CTA's warps read it: one of them works it out, the others would have its code in the instruction cache besides (with it in every role the kernel
-// was 192 KB long, and the products stood still for instructions).
-struct Work {
-  int units;       // that have keys; -1: there is no more
-  int turns;       // both sets hold the same rows and take the units in turn
-  int count[2];    // each set's units
-  int first;       // the part's first unit in its tile
-  int b, key_row;  // sequence, and the key head's first row in a page
-  int keys, pos0, tok0, rows;  // as in Part
-  int head0, heads;
-  int slot;        // of its sums, -1: the tile is whole
-  int pad[2];
-};
-constexpr int kRingWorks = 8;
-
 template <int D> struct Shape {
   static constexpr int kHalves = D / 64;
   static constexpr int kTile = kHalves * kHalf;
@@ -100,31 +85,18 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long s, float a
 __device__ __forceinline__ float lo2(unsigned long long s) { return __uint_as_float((uint32_t)s); }
 __device__ __forceinline__ float hi2(unsigned long long s) { return __uint_as_float((uint32_t)(s >> 32)); }
 
-__device__ __forceinline__ Work work_of(const Params& p, const Part& t, int slot) {
+// How a part's units fall to the two sets.
+__device__ __forceinline__ void share_out(const Params& p, Work* w) {
   const int tokens = p.split.tile_tokens / 2;  // of a set
-  Work w;
-  w.turns = t.rows <= tokens * p.split.block_heads;
-  w.units = max(0, min(t.take, (t.keys + kUnit - 1) / kUnit - (int)t.first));
-  if (w.turns) {
-    w.count[0] = (w.units + 1) / 2;
-    w.count[1] = w.units / 2;
+  w->turns = w->rows <= tokens * p.split.block_heads;
+  if (w->turns) {
+    w->count[0] = (w->units + 1) / 2;
+    w->count[1] = w->units / 2;
   } else {
-    const int keys = p.split.causal ? min(t.pos0 + tokens, t.keys) : t.keys;
-    w.count[0] = max(0, min(w.units, (keys + kUnit - 1) / kUnit - (int)t.first));
-    w.count[1] = w.units;
+    const int keys = p.split.causal ? min(w->pos0 + tokens, w->keys) : w->keys;
+    w->count[0] = max(0, min(w->units, (keys + kUnit - 1) / kUnit - w->first));
+    w->count[1] = w->units;
   }
-  w.first = (int)t.first;
-  w.b = t.b;
-  w.key_row = t.block / p.split.head_blocks << p.s.page_shift;
-  w.keys = t.keys;
-  w.pos0 = t.pos0;
-  w.tok0 = t.tok0;
-  w.rows = t.rows;
-  w.head0 = first_head(p, t.block);
-  w.heads = heads_of(p, t.block);
-  w.slot = t.take == t.units ? -1 : slot;
-  w.pad[0] = w.pad[1] = 0;
-  return w;
 }
 
 template <typename T, int D>
@@ -210,7 +182,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       uint32_t used[2] = {0, 0}, parity[2] = {0, 0};  // a bit for each slot: whether the set reads what is there, and the phase of its kv_empty
       bool ok = true, both = false;                   // both: the second set reads the first queries' buffer too
       // The first loader works the parts out, one ahead of its own loads.
-      Part t;
+      Part t = {};
       long long u = lo;
       bool cut_here = false;
       auto publish = [&](Work* w) {
@@ -220,6 +192,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (n > 0) next_part(p, t, hi - u);
           else t = part_at(p, prefix, lo, hi - lo);
           *w = work_of(p, t, 2 * cta + (u == lo ? 0 : 1));
+          share_out(p, w);
           if (w->slot >= 0 && t.first == 0) {
             cut_here = true;
             if (lane == 0) p.parts.cuts[cta] = cut_of(p, t, u, total, cta, ctas, w->slot);

@@ -77,10 +77,10 @@ struct Split {
   int block_heads;  // query heads of a tile
   int blocks;       // head blocks of a sequence, over all key heads
   int head_blocks;  // of them a key head's
-  int tile_tokens, unit, causal;
+  int tile_tokens, unit_shift, causal;
 };
 
-// `rows` rows a tile of `parts` separate sets: a set's rows are whole tokens.
+// `rows` rows a tile of `parts` separate sets: a set's rows are whole tokens. `unit` is a power of two.
 TTB_PAGED_FN Split split_of(int heads, int kv_heads, int rows, int parts, int unit, int causal) {
   Split s;
   const int group = heads / kv_heads;
@@ -89,25 +89,34 @@ TTB_PAGED_FN Split split_of(int heads, int kv_heads, int rows, int parts, int un
   s.head_blocks = (group + s.block_heads - 1) / s.block_heads;  // (none of them empty)
   s.blocks = kv_heads * s.head_blocks;
   s.tile_tokens = rows / s.block_heads * parts;
-  s.unit = unit;
+  s.unit_shift = 0;
+  while ((1 << s.unit_shift) < unit) ++s.unit_shift;
   s.causal = causal;
   return s;
 }
 
-TTB_PAGED_FN int64_t tiles_of(const Split& s, int64_t n) { return (n + s.tile_tokens - 1) / s.tile_tokens; }
+// A quotient of numbers that are not negative: of 32 bits where they fit, which takes a tenth of the instructions.
+TTB_PAGED_FN int64_t quotient(int64_t a, int64_t b) { return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b; }
 
-// units of one head block of tile t: of the keys that its last token sees
+TTB_PAGED_FN int64_t tiles_of(const Split& s, int64_t n) { return quotient(n + s.tile_tokens - 1, s.tile_tokens); }
+
+// units of `keys` keys
+TTB_PAGED_FN int64_t units_of(const Split& s, int64_t keys) { return (keys + (1 << s.unit_shift) - 1) >> s.unit_shift; }
+
+// of one head block of tile t: of the keys that its last token sees
 TTB_PAGED_FN int64_t units_of_tile(const Split& s, int64_t past, int64_t n, int64_t t) {
   const int64_t end = (t + 1) * s.tile_tokens;
-  return (past + (s.causal && end < n ? end : n) + s.unit - 1) / s.unit;
+  return units_of(s, past + (s.causal && end < n ? end : n));
 }
 
 // of the tiles before t together (t at most tiles_of)
 TTB_PAGED_FN int64_t units_before_tile(const Split& s, int64_t past, int64_t n, int64_t t) {
-  if (!s.causal) return t * ((past + n + s.unit - 1) / s.unit);
-  const int64_t whole = n / s.tile_tokens;  // tiles whose last token is not the sequence's
+  if (t == 0) return 0;
+  const int64_t all = units_of(s, past + n);
+  if (!s.causal || n <= s.tile_tokens) return t * all;
+  const int64_t whole = quotient(n, s.tile_tokens);  // tiles whose last token is not the sequence's
   const int64_t m = t < whole ? t : whole;
-  return floor_sum(m, s.unit, s.tile_tokens, past + s.tile_tokens + s.unit - 1) + (t > m ? (past + n + s.unit - 1) / s.unit : 0);
+  return floor_sum(m, 1 << s.unit_shift, s.tile_tokens, past + s.tile_tokens + (1 << s.unit_shift) - 1) + (t > m ? all : 0);
 }
 
 TTB_PAGED_FN int64_t units_of_sequence(const Split& s, int64_t past, int64_t n) { return n > 0 ? units_before_tile(s, past, n, tiles_of(s, n)) * s.blocks : 0; }
@@ -131,17 +140,17 @@ TTB_PAGED_FN Place place_of(const Split& s, int64_t past, int64_t n, int64_t x) 
   p.tile = lo;
   x -= lo ? units_before_tile(s, past, n, lo) * s.blocks : 0;
   p.units = units_of_tile(s, past, n, lo);
-  p.block = (int)(x / p.units);
+  p.block = (int)quotient(x, p.units);
   p.first = x - p.block * p.units;
   return p;
 }
 
 // CTAs that share a line of `units`, at least `least` units each; and where the stretch of CTA c begins.
 TTB_PAGED_FN int ctas_of(int64_t units, int ctas, int least) {
-  const int64_t n = (units + least - 1) / least;
+  const int64_t n = quotient(units + least - 1, least);
   return n < ctas ? (int)n : ctas;
 }
-TTB_PAGED_FN int64_t first_unit(int64_t units, int ctas, int c) { return units * c / ctas; }
+TTB_PAGED_FN int64_t first_unit(int64_t units, int ctas, int c) { return quotient(units * c, ctas); }
 
 }  // namespace paged
 }  // namespace ttb

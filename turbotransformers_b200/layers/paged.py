@@ -34,7 +34,14 @@ def _fail(name, why):
     raise ValueError(f"{name} {why}")
 
 
-def _rows(t, name, d=None):
+def _gpu(t, name):
+    device = t.get_device()
+    if device < 0:
+        raise RuntimeError(f"{name} is not on a CUDA device: this runtime has no CPU path")
+    return device
+
+
+def _rows(t, name, device, dtype, d=None):
     """(rows, heads, head size, elements between rows) of a [tokens, heads, d] tensor whose heads lie side by side."""
     if t.dim() != 3:
         _fail(name, "must be [tokens, heads, head size]")
@@ -43,50 +50,53 @@ def _rows(t, name, d=None):
         _fail(name, "must have its heads side by side (strides [any, head size, 1])")
     if d is not None and width != d:
         _fail(name, f"must have heads of {d}")
+    if t.dtype != dtype or t.get_device() != device:
+        _fail(name, f"must be {dtype} on cuda:{device}")
     return n, heads, width, row if n > 1 else heads * width
 
 
-def _same(device, **tensors):
-    for name, t in tensors.items():
-        if t.device != device:
-            _fail(name, f"is on {t.device}, not on {device}")
+def _like(out, x, name, device):
+    """Elements between rows of an output, which has its input's shape, dtype and device."""
+    if out.shape != x.shape:
+        _fail(name, "must be like its input")
+    return _rows(out, name, device, x.dtype)[3]
 
 
-def _index(t, name, shape, device, dtype=torch.int32):
-    if t.dtype != dtype or not t.is_contiguous() or t.device != device or tuple(t.shape) != shape:
-        _fail(name, f"must be a contiguous {dtype} tensor of {list(shape)} on {device}")
+def _index(t, name, n, device, dtype=torch.int32):
+    if t.dtype != dtype or t.get_device() != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        _fail(name, f"must be a contiguous {dtype} vector of {n} on cuda:{device}")
     return t.data_ptr()
 
 
-def _gpu(t, name):
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} is not on a CUDA device: this runtime has no CPU path")
-    return t.device.index
-
-
 def _freqs(freqs, device):
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or freqs.device != device:
-        _fail("freqs", f"must be a contiguous float64 vector on {device}")
-    return freqs.data_ptr(), 2 * freqs.numel()
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or freqs.get_device() != device:
+        _fail("freqs", f"must be a contiguous float64 vector on cuda:{device}")
+    return freqs.data_ptr(), 2 * freqs.shape[0]
+
+
+def _table(table, device):
+    """(address, elements between rows, rows, width) of a page table."""
+    if table.dim() != 2 or table.dtype != torch.int32 or table.get_device() != device:
+        _fail("table", f"must be int32 [sequences, pages] on cuda:{device}")
+    (B, width), (row, one) = table.shape, table.stride()
+    if one != 1 and width > 1:
+        _fail("table", "must have contiguous rows")
+    return table.data_ptr(), row if B > 1 else width, B, width
 
 
 def _kv(keys, values, table, cu_seqlens, past_lens, dtype, device):
     """The arguments that describe one layer's pages."""
-    if keys.dim() != 4 or keys.shape != values.shape:
+    shape, strides = keys.shape, keys.stride()
+    if len(shape) != 4 or shape != values.shape:
         _fail("keys and values", "must be [pages, key heads, page tokens, head size], alike")
-    if keys.dtype != dtype or values.dtype != dtype:
-        _fail("keys and values", f"must be {dtype}, as the rows are")
-    _same(device, keys=keys, values=values, table=table)
-    pages, heads, tokens, d = keys.shape
-    strides = keys.stride()
+    if keys.dtype != dtype or values.dtype != dtype or keys.get_device() != device or values.get_device() != device:
+        _fail("keys and values", f"must be {dtype} on cuda:{device}, as the rows are")
+    pages, heads, tokens, d = shape
     if strides != values.stride() or strides[1:] != (tokens * d, d, 1):
         _fail("keys and values", "must have contiguous pages, equally far apart")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 and table.shape[1] > 1:
-        _fail("table", "must be int32 [sequences, pages] with contiguous rows")
-    B, width = table.shape
-    cu, past = _index(cu_seqlens, "cu_seqlens", (B + 1,), device), _index(past_lens, "past_lens", (B,), device)
-    return (keys.data_ptr(), values.data_ptr(), strides[0] if pages > 1 else heads * tokens * d, pages, heads, tokens, d, table.data_ptr(),
-            table.stride(0) if B > 1 else width, width, cu, past, B)
+    at, row, B, width = _table(table, device)
+    return (keys.data_ptr(), values.data_ptr(), strides[0] if pages > 1 else heads * tokens * d, pages, heads, tokens, d, at, row, width,
+            _index(cu_seqlens, "cu_seqlens", B + 1, device), _index(past_lens, "past_lens", B, device), B)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
@@ -94,29 +104,28 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     """Rotary positions of q [tokens, heads, d] and k [tokens, key heads, d] (or None): returns (q, k) turned, in new tensors or in `out` (which may be (q, k)
     themselves). positions: int64 [tokens]. freqs: float64 [n], radians a position; the first 2n elements of every head are turned, in pairs (i, i + n), or (2i, 2i + 1) if
     interleaved, and their length is multiplied by scale."""
-    device = _gpu(q, "q")
-    if q.dtype not in _CODE:
+    device, dtype = _gpu(q, "q"), q.dtype
+    if dtype not in _CODE:
         _fail("q", "must be fp32, fp16 or bf16")
-    T, heads, d, ldq = _rows(q, "q")
-    at, turned = _freqs(freqs, q.device)
-    where = _index(positions, "positions", (T,), q.device, torch.int64)
-    kv_heads = ldk = 0
+    T, heads, d, ldq = _rows(q, "q", device, dtype)
+    at, turned = _freqs(freqs, device)
+    where = _index(positions, "positions", T, device, torch.int64)
+    kp = kv_heads = ldk = 0
     if k is not None:
-        n, kv_heads, _, ldk = _rows(k, "k", d)
-        if n != T or k.dtype != q.dtype:
-            _fail("k", "must have q's tokens and dtype")
-        _same(q.device, k=k)
+        n, kv_heads, _, ldk = _rows(k, "k", device, dtype, d)
+        if n != T:
+            _fail("k", "must have q's tokens")
+        kp = k.data_ptr()
     if out is None:
-        q_out, k_out = torch.empty((T, heads, d), dtype=q.dtype, device=q.device), None if k is None else torch.empty((T, kv_heads, d), dtype=q.dtype, device=q.device)
+        q_out, k_out = torch.empty_like(q), None if k is None else torch.empty_like(k)
         ldq_out, ldk_out = heads * d, kv_heads * d
     else:
         q_out, k_out = out
-        for o, x, name in ((q_out, q, "out[0]"), (k_out, k, "out[1]")):
-            if (o is None) != (x is None) or o is not None and (o.shape != x.shape or o.dtype != x.dtype or o.device != x.device):
-                _fail(name, "must be like its input")
-        ldq_out, ldk_out = _rows(q_out, "out[0]")[3], 0 if k is None else _rows(k_out, "out[1]")[3]
-    cxx.rotary(device, _stream(device), _CODE[q.dtype], q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
-               ldq, ldk, ldq_out, ldk_out, T, heads, kv_heads, d, turned, where, at, interleaved, scale)
+        if (k_out is None) != (k is None):
+            _fail("out", "must have keys where there are keys")
+        ldq_out, ldk_out = _like(q_out, q, "out[0]", device), 0 if k is None else _like(k_out, k, "out[1]", device)
+    cxx.rotary(device, _stream(device), _CODE[dtype], q.data_ptr(), kp, q_out.data_ptr(), kp and k_out.data_ptr(), ldq, ldk, ldq_out, ldk_out, T, heads, kv_heads, d,
+               turned, where, at, interleaved, scale)
     return q_out, k_out
 
 
@@ -126,36 +135,33 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: t
     """Files k and v [tokens, key heads, d] of new tokens as tokens past_lens[b] and following of their sequences. Sequence b's are rows cu_seqlens[b] to
     cu_seqlens[b + 1]; table int32 [sequences, width] lists the pages of each; keys and values are the layer's pool [pages, key heads, page tokens, d]. With `freqs` (see
     rotary) the keys are turned by their places on the way, and so is q, which is returned in a new tensor or in `out`."""
-    device = _gpu(k, "k")
-    if k.dtype not in _CODE:
+    device, dtype = _gpu(k, "k"), k.dtype
+    if dtype not in _CODE:
         _fail("k", "must be fp16 or bf16")
-    T, heads, d, ldk = _rows(k, "k")
-    n, other, _, ldv = _rows(v, "v", d)
-    if n != T or other != heads or v.dtype != k.dtype:
+    T, heads, d, ldk = _rows(k, "k", device, dtype)
+    n, other, _, ldv = _rows(v, "v", device, dtype, d)
+    if n != T or other != heads:
         _fail("v", "must be like k")
-    kv = _kv(keys, values, table, cu_seqlens, past_lens, k.dtype, k.device)
+    kv = _kv(keys, values, table, cu_seqlens, past_lens, dtype, device)
     if kv[4] != heads or kv[6] != d:
         _fail("k", "must have the pool's heads")
-    _same(k.device, v=v)
     if freqs is None:
         if q is not None:
             _fail("q", "is turned by freqs: it has none without them")
-        cxx.paged_append(device, _stream(device), _CODE[k.dtype], *kv, T, k.data_ptr(), ldk, v.data_ptr(), ldv, 0, 0, False, 1.0, 0, 0, 0, 0, 0)
+        cxx.paged_append(device, _stream(device), _CODE[dtype], *kv, T, k.data_ptr(), ldk, v.data_ptr(), ldv, 0, 0, False, 1.0, 0, 0, 0, 0, 0)
         return None
-    at, turned = _freqs(freqs, k.device)
+    at, turned = _freqs(freqs, device)
     qp = op = ldq = ldq_out = q_heads = 0
     if q is not None:
-        n, q_heads, _, ldq = _rows(q, "q", d)
-        if n != T or q.dtype != k.dtype:
-            _fail("q", "must have k's tokens and dtype")
-        _same(k.device, q=q)
+        n, q_heads, _, ldq = _rows(q, "q", device, dtype, d)
+        if n != T:
+            _fail("q", "must have k's tokens")
         if out is None:
-            out = torch.empty((T, q_heads, d), dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-            _fail("out", "must be like q")
-        qp, op, ldq_out = q.data_ptr(), out.data_ptr(), _rows(out, "out")[3]
-    cxx.paged_append(device, _stream(device), _CODE[k.dtype], *kv, T, k.data_ptr(), ldk, v.data_ptr(), ldv, at, turned, interleaved, scale, qp, op, ldq, ldq_out,
-                     q_heads)
+            out, ldq_out = torch.empty_like(q), q_heads * d
+        else:
+            ldq_out = _like(out, q, "out", device)
+        qp, op = q.data_ptr(), out.data_ptr()
+    cxx.paged_append(device, _stream(device), _CODE[dtype], *kv, T, k.data_ptr(), ldk, v.data_ptr(), ldv, at, turned, interleaved, scale, qp, op, ldq, ldq_out, q_heads)
     return out if q is not None else None
 
 
@@ -164,44 +170,42 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
     """Attention of q [tokens, heads, d] over the pages of its sequences (arguments as for paged_append, whose new tokens have been filed): token i of a sequence sees its
     cached tokens up to itself, or all past + new of them if not causal. heads is a multiple of the key heads; scale is d ** -0.5 unless given. Rows that belong to no sequence
     are left as they are in `out`, undefined without it."""
-    device = _gpu(q, "q")
-    if q.dtype not in _CODE:
+    device, dtype = _gpu(q, "q"), q.dtype
+    if dtype not in _CODE:
         _fail("q", "must be fp16 or bf16")
-    T, heads, d, ldq = _rows(q, "q")
-    kv = _kv(keys, values, table, cu_seqlens, past_lens, q.dtype, q.device)
+    T, heads, d, ldq = _rows(q, "q", device, dtype)
+    kv = _kv(keys, values, table, cu_seqlens, past_lens, dtype, device)
     if kv[6] != d or heads % max(kv[4], 1):
         _fail("q", "must have the pool's head size, and a multiple of its heads")
     if out is None:
-        out = torch.empty((T, heads, d), dtype=q.dtype, device=q.device)
-        ldo = heads * d
+        out, ldo = torch.empty_like(q), heads * d
     else:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
-            _fail("out", "must be like q")
-        ldo = _rows(out, "out")[3]
-    cxx.paged_attention(device, _stream(device), _CODE[q.dtype], *kv, q.data_ptr(), ldq, T, heads, causal, d ** -0.5 if scale is None else scale, out.data_ptr(), ldo)
+        ldo = _like(out, q, "out", device)
+    cxx.paged_attention(device, _stream(device), _CODE[dtype], *kv, q.data_ptr(), ldq, T, heads, causal, d ** -0.5 if scale is None else scale, out.data_ptr(), ldo)
     return out
 
 
 def _tables(table, lens, refs):
     device = _gpu(table, "table")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1 and table.shape[1] > 1:
-        _fail("table", "must be int32 [sequences, pages] with contiguous rows")
-    B, width = table.shape
+    t = _table(table, device)
     if refs.dim() != 1:
         _fail("refs", "must be a vector")
-    return device, (table.data_ptr(), table.stride(0) if B > 1 else width, B, width, 0 if lens is None else _index(lens, "lens", (B,), table.device),
-                    _index(refs, "refs", tuple(refs.shape), table.device), refs.numel())
+    pages = refs.shape[0]
+    return device, t + (0 if lens is None else _index(lens, "lens", t[2], device), _index(refs, "refs", pages, device), pages)
 
 
 def _pool(pool):
-    if pool.dim() < 3:
+    shape, strides = pool.shape, pool.stride()
+    if len(shape) < 3:
         _fail("pool", "must be [planes, pages, ...]")
-    if not pool[0, 0].is_contiguous():
-        _fail("pool", "must have contiguous pages")
-    size, (planes, pages) = pool.element_size(), pool.shape[:2]
-    page = size * math.prod(pool.shape[2:])
-    page_stride = pool.stride(1) * size if pages > 1 else page
-    return pool.data_ptr(), planes, pool.stride(0) * size if planes > 1 else pages * page_stride, pages, page_stride, page
+    page = 1
+    for n, stride in zip(reversed(shape[2:]), reversed(strides[2:])):
+        if stride != page and n > 1:
+            _fail("pool", "must have contiguous pages")
+        page *= n
+    size, planes, pages = pool.element_size(), shape[0], shape[1]
+    page_stride = strides[1] if pages > 1 else page
+    return pool.data_ptr(), planes, size * (strides[0] if planes > 1 else pages * page_stride), pages, size * page_stride, size * page
 
 
 def paged_reserve(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, new_tokens: torch.Tensor, page_tokens: int):
@@ -209,8 +213,8 @@ def paged_reserve(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, n
     page that other rows list too gets one of its own in its place. Returns (granted int32 [sequences], copies int32 [sequences, 2]); hand the copies to paged_copy before the new
     tokens are filed. A row that is not granted (0) has been left alone: the pool is full, or its row of the table."""
     device, t = _tables(table, lens, refs)
-    new = _index(new_tokens, "new_tokens", (t[2],), table.device)
-    granted, copies = torch.empty(t[2], dtype=torch.int32, device=table.device), torch.empty((t[2], 2), dtype=torch.int32, device=table.device)
+    new = _index(new_tokens, "new_tokens", t[2], device)
+    granted, copies = torch.empty_like(new_tokens), new_tokens.new_empty((t[2], 2))
     cxx.paged_reserve(device, _stream(device), *t, new, page_tokens, granted.data_ptr(), copies.data_ptr())
     return granted, copies
 
@@ -218,23 +222,24 @@ def paged_reserve(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, n
 def paged_fork(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor) -> None:
     """Row b of the page table becomes what row parents[b] was, and shares its pages; parents[b] = -1 frees the row. table, lens and refs are changed in place."""
     device, t = _tables(table, lens, refs)
-    cxx.paged_fork(device, _stream(device), *t, _index(parents, "parents", (t[2],), table.device))
+    cxx.paged_fork(device, _stream(device), *t, _index(parents, "parents", t[2], device))
 
 
 def paged_copy(pool: torch.Tensor, pairs: torch.Tensor) -> None:
     """Page pairs[i, 1] of every plane of pool [planes, pages, ...] becomes a copy of page pairs[i, 0] (int32 [n, 2]; pairs with a negative entry are left out). A page that
     is written may not be in another pair."""
     device = _gpu(pool, "pool")
-    if pairs.dim() != 2:
-        _fail("pairs", "must be [n, 2]")
-    cxx.paged_copy(device, _stream(device), *_pool(pool), _index(pairs, "pairs", (pairs.shape[0], 2), pool.device), pairs.shape[0])
+    if pairs.dim() != 2 or pairs.shape[1] != 2 or pairs.dtype != torch.int32 or pairs.get_device() != device or not pairs.is_contiguous():
+        _fail("pairs", f"must be a contiguous int32 [n, 2] on cuda:{device}")
+    cxx.paged_copy(device, _stream(device), *_pool(pool), pairs.data_ptr(), pairs.shape[0])
 
 
 def paged_compact(table: torch.Tensor, refs: torch.Tensor, pool: torch.Tensor) -> torch.Tensor:
     """Moves the pages in use to the front of the pool, table and refs with them. Returns how many there are (int32 [1] on the device)."""
     device, t = _tables(table, None, refs)
-    _same(table.device, pool=pool)
-    used = torch.empty(1, dtype=torch.int32, device=table.device)
+    if pool.get_device() != device:
+        _fail("pool", f"must be on cuda:{device}")
+    used = refs.new_empty(1)
     cxx.paged_compact(device, _stream(device), *t, *_pool(pool), used.data_ptr())
     return used
 
