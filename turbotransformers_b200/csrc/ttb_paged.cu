@@ -17,12 +17,16 @@ namespace {
 // of its own over both, and a launch, saved.
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryTokens = 8;  // of a block, at most
+constexpr int kRotaryUnits = 2;   // that a thread has on their way
 
 struct RotaryParams {
   const void *q, *k, *v;
   void *q_out, *k_out;
   long long ldq, ldk, ldv, ldq_out, ldk_out;
   int tokens, heads, kv_heads, d, half, interleaved, block_tokens;
+  int rows;                 // heads of a token, all together
+  unsigned per;             // units of a head
+  unsigned per_magic, rows_magic;  // their reciprocals, times 2^32 and rounded up; rows_magic is 0 for blocks of one token
   float scale;
   const int64_t* positions;
   const double* freqs;
@@ -41,62 +45,119 @@ __device__ __forceinline__ int sequence_at(const Sequences& s, int t, int lane) 
   return lo + __popc(__ballot_sync(0xffffffffu, i < lo + step && i <= s.B && s.cu[min(i, s.B)] <= t));
 }
 
-// One unit of a head, in place or not: WIDE, eight pairs (halves) or four (neighbours), or eight elements that are not turned; else a pair or an element.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void turn_unit(const T* src, T* dst, int unit, int half, int interleaved, const float2* cs) {
-  if (WIDE) {
-    if (interleaved) {
-      Vec8<T> x;
-      x.load(src + unit * 8);
-      if (unit * 4 < half) {
+// What a thread turns at a time: WIDE, eight pairs (halves) or four (neighbours), or eight elements that are not turned; else a pair or an element.
+template <typename T, bool WIDE> struct Piece;
+template <typename T> struct Piece<T, true> {
+  static constexpr int kWords = sizeof(T) / 2;  // of 16 bytes
+  uint4 w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 c = cs[unit * 4 + e];
-          const float a = x.v[2 * e], b = x.v[2 * e + 1];
-          x.v[2 * e] = a * c.x - b * c.y;
-          x.v[2 * e + 1] = b * c.x + a * c.y;
-        }
-      }
-      x.store(dst + unit * 8);
-    } else if (unit * 8 < half) {
-      Vec8<T> x, y;
-      x.load(src + unit * 8);
-      y.load(src + half + unit * 8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 c = cs[unit * 8 + e];
-        const float a = x.v[e], b = y.v[e];
-        x.v[e] = a * c.x - b * c.y;
-        y.v[e] = b * c.x + a * c.y;
-      }
-      x.store(dst + unit * 8);
-      y.store(dst + half + unit * 8);
-    } else {
-      Vec8<T> x;
-      x.load(src + half + unit * 8);
-      x.store(dst + half + unit * 8);
-    }
-  } else if (unit < half) {
-    const int i = interleaved ? 2 * unit : unit, j = interleaved ? 2 * unit + 1 : unit + half;
-    const float a = to_f(src[i]), b = to_f(src[j]);
-    const float2 c = cs[unit];
-    dst[i] = from_f<T>(a * c.x - b * c.y);
-    dst[j] = from_f<T>(b * c.x + a * c.y);
-  } else {
-    dst[half + unit] = src[half + unit];
+    for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
   }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(p)[i] = w[i];
+  }
+};
+template <typename T> struct Piece<T, false> {
+  T w;
+  __device__ __forceinline__ void load(const T* p) { w = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = w; }
+};
+
+// Where unit `idx` of a block lies: its token, its head among the token's query, key and (PAGED) value heads, its elements `first` and (a pair of halves)
+// `second`, else -1, and its first pair, -1 where nothing is turned. Every head has the same units, those of the values too.
+struct UnitPlace {
+  int token, head, first, second, pair;
+};
+template <bool WIDE>
+__device__ __forceinline__ UnitPlace unit_place(const RotaryParams& p, unsigned idx) {
+  UnitPlace w;
+  // WIDE: at most 64 units of 196605 heads, so that the rounded-up reciprocals are exact (their error times idx stays below 2^32); blocks of more than one
+  // token are small. Plain divisions of both took half of the kernel's instructions.
+  const unsigned row = !WIDE ? idx / p.per : p.per == 1 ? idx : __umulhi(idx, p.per_magic);
+  w.token = p.rows == 1 ? (int)row : (int)__umulhi(row, p.rows_magic);
+  w.head = (int)(row - w.token * (unsigned)p.rows);
+  const int u = (int)(idx - row * p.per), wide = WIDE ? 8 : 1;
+  w.second = -1;
+  if (WIDE && p.interleaved) {
+    w.first = u * 8;
+    w.pair = u * 4 < p.half ? u * 4 : -1;
+  } else if (u * wide < p.half) {
+    w.first = p.interleaved ? 2 * u : u * wide;
+    w.second = p.interleaved ? 2 * u + 1 : p.half + u * wide;
+    w.pair = u * wide;
+  } else {
+    w.first = p.half + u * wide;
+    w.pair = -1;
+  }
+  return w;
+}
+
+template <typename T>
+__device__ __forceinline__ void turn(Piece<T, true>& x, Piece<T, true>& y, bool halves, const float2* cs) {
+  Vec8<T> a, b;
+  a.load(reinterpret_cast<const T*>(x.w));
+  if (halves) {
+    b.load(reinterpret_cast<const T*>(y.w));
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float4 c = *reinterpret_cast<const float4*>(cs + e);
+      const float f = a.v[e], g = b.v[e], h = a.v[e + 1], i = b.v[e + 1];
+      a.v[e] = f * c.x - g * c.y;
+      b.v[e] = g * c.x + f * c.y;
+      a.v[e + 1] = h * c.z - i * c.w;
+      b.v[e + 1] = i * c.z + h * c.w;
+    }
+    b.store(reinterpret_cast<T*>(y.w));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const float4 c = *reinterpret_cast<const float4*>(cs + e);
+      const float f = a.v[2 * e], g = a.v[2 * e + 1], h = a.v[2 * e + 2], i = a.v[2 * e + 3];
+      a.v[2 * e] = f * c.x - g * c.y;
+      a.v[2 * e + 1] = g * c.x + f * c.y;
+      a.v[2 * e + 2] = h * c.z - i * c.w;
+      a.v[2 * e + 3] = i * c.z + h * c.w;
+    }
+  }
+  a.store(reinterpret_cast<T*>(x.w));
+}
+template <typename T>
+__device__ __forceinline__ void turn(Piece<T, false>& x, Piece<T, false>& y, bool, const float2* cs) {
+  const float f = to_f(x.w), g = to_f(y.w);
+  x.w = from_f<T>(f * cs->x - g * cs->y);
+  y.w = from_f<T>(g * cs->x + f * cs->y);
 }
 
 template <typename T, bool WIDE, bool PAGED>
-__global__ void __launch_bounds__(kRotaryThreads)
+__global__ void __launch_bounds__(kRotaryThreads, sizeof(T) == 2 ? 6 : 4)
 rotary_kernel(const RotaryParams p) {
-  extern __shared__ float2 cs[];  // [block_tokens][half]
+  extern __shared__ __align__(16) float2 cs[];  // [block_tokens][half]
   __shared__ double s_pos[kRotaryTokens];
   __shared__ long long s_page[kRotaryTokens];  // PAGED: the token's first element of the pools, -1: it has no place
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int t0 = blockIdx.x * p.block_tokens, n = min(p.block_tokens, p.tokens - t0);
+  const int units = n * p.rows * (int)p.per;
+  Piece<T, WIDE> x[kRotaryUnits], y[kRotaryUnits];
+  auto load = [&](int idx0) {
+#pragma unroll
+    for (int b = 0; b < kRotaryUnits; ++b) {
+      const int idx = idx0 + b * kRotaryThreads;
+      if (idx >= units) break;
+      const UnitPlace w = unit_place<WIDE>(p, idx);
+      const long long t = t0 + w.token;
+      const T* src;
+      if (w.head < p.heads) src = static_cast<const T*>(p.q) + t * p.ldq + w.head * p.d;
+      else if (!PAGED || w.head < p.heads + p.kv_heads) src = static_cast<const T*>(p.k) + t * p.ldk + (w.head - p.heads) * p.d;
+      else src = static_cast<const T*>(p.v) + t * p.ldv + (w.head - p.heads - p.kv_heads) * p.d;
+      x[b].load(src + w.first);
+      if (w.second >= 0) y[b].load(src + w.second);
+    }
+  };
+  load(tid);  // on their way while the block works out its positions
   for (int i = PAGED ? warp : tid; i < n; i += PAGED ? kRotaryThreads / 32 : kRotaryThreads) {
     const int t = t0 + i;
     if (!PAGED) {
@@ -132,35 +193,26 @@ rotary_kernel(const RotaryParams p) {
     cs[i] = make_float2(c * p.scale, s * p.scale);
   }
   __syncthreads();
-  // units of a head, of a token's queries, its keys, and (PAGED) its values
-  const int wide = p.interleaved ? p.d / 8 : (p.d - p.half) / 8;
-  const int per = WIDE ? wide : p.d - p.half, qn = p.heads * per, kn = p.kv_heads * per, vn = PAGED ? p.kv_heads * p.d / (WIDE ? 8 : 1) : 0;
-  const int each = qn + kn + vn;
-  for (int idx = tid; idx < n * each; idx += kRotaryThreads) {
-    const int i = idx / each, u = idx - i * each, t = t0 + i;
-    const float2* c = cs + i * p.half;
-    if (u < qn) {
-      if (PAGED && s_pos[i] < 0) continue;
-      const int h = u / per;
-      turn_unit<T, WIDE>(static_cast<const T*>(p.q) + t * p.ldq + h * p.d, static_cast<T*>(p.q_out) + t * p.ldq_out + h * p.d, u - h * per, p.half, p.interleaved, c);
-    } else if (u < qn + kn) {
-      if (PAGED && s_page[i] < 0) continue;
-      const int h = (u - qn) / per;
-      T* dst = PAGED ? static_cast<T*>(p.keys) + s_page[i] + ((long long)h << p.s.page_shift) * p.d : static_cast<T*>(p.k_out) + t * p.ldk_out + h * p.d;
-      turn_unit<T, WIDE>(static_cast<const T*>(p.k) + t * p.ldk + h * p.d, dst, u - qn - h * per, p.half, p.interleaved, c);
-    } else if (PAGED) {
-      if (s_page[i] < 0) continue;
-      const int w = WIDE ? p.d / 8 : p.d, h = (u - qn - kn) / w, e = (u - qn - kn - h * w) * (p.d / w);
-      const T* src = static_cast<const T*>(p.v) + t * p.ldv + h * p.d + e;
-      T* dst = static_cast<T*>(p.values) + s_page[i] + ((long long)h << p.s.page_shift) * p.d + e;
-      if (WIDE) {
-        Vec8<T> x;
-        x.load(src);
-        x.store(dst);
-      } else {
-        *dst = *src;
-      }
+
+  for (int idx0 = tid; idx0 < units;) {
+#pragma unroll
+    for (int b = 0; b < kRotaryUnits; ++b) {
+      const int idx = idx0 + b * kRotaryThreads;
+      if (idx >= units) break;
+      const UnitPlace w = unit_place<WIDE>(p, idx);
+      const bool query = w.head < p.heads, key = w.head < p.heads + p.kv_heads;
+      if (PAGED && (query ? s_pos[w.token] < 0 : s_page[w.token] < 0)) continue;
+      if (w.pair >= 0 && (!PAGED || key)) turn(x[b], y[b], w.second >= 0, cs + w.token * p.half + w.pair);
+      const long long t = t0 + w.token;
+      T* dst;
+      if (query) dst = static_cast<T*>(p.q_out) + t * p.ldq_out + w.head * p.d;
+      else if (!PAGED) dst = static_cast<T*>(p.k_out) + t * p.ldk_out + (w.head - p.heads) * p.d;
+      else dst = static_cast<T*>(key ? p.keys : p.values) + s_page[w.token] + (((long long)w.head - p.heads - (key ? 0 : p.kv_heads)) << p.s.page_shift) * p.d;
+      x[b].store(dst + w.first);
+      if (w.second >= 0) y[b].store(dst + w.second);
     }
+    idx0 += kRotaryUnits * kRotaryThreads;
+    load(idx0);
   }
 }
 
@@ -170,8 +222,12 @@ int launch_rotary(ttb_ctx* ctx, RotaryParams& p, const char* what) {
                        reinterpret_cast<uintptr_t>(p.q_out) | reinterpret_cast<uintptr_t>(p.k_out);
   const bool wide = (at & 15) == 0 && ((p.ldq | p.ldk | p.ldv | p.ldq_out | p.ldk_out) * (int)sizeof(T)) % 16 == 0 && p.half % (p.interleaved ? 4 : 8) == 0;
   // tokens of a block: enough for every thread to have some units, few enough for the tokens to reach all SMs
-  const int units = (p.heads + (PAGED ? 2 : 1) * p.kv_heads) * p.d / 16;
-  p.block_tokens = std::max(1, std::min(std::min(kRotaryTokens, 4 * kRotaryThreads / std::max(1, units)), p.tokens / (4 * ctx->sm_count)));
+  p.rows = p.heads + (PAGED ? 2 : 1) * p.kv_heads;
+  p.per = !wide ? p.d - p.half : p.interleaved ? p.d / 8 : (p.d - p.half) / 8;
+  const int units = p.rows * p.d / 16;
+  p.block_tokens = std::max(1, std::min(std::min(kRotaryTokens, 2 * kRotaryUnits * kRotaryThreads / std::max(1, units)), p.tokens / (4 * ctx->sm_count)));
+  p.per_magic = (unsigned)(((1ull << 32) + p.per - 1) / p.per);
+  p.rows_magic = p.block_tokens == 1 ? 0 : (unsigned)(((1ull << 32) + p.rows - 1) / p.rows);
   const dim3 grid((unsigned)((p.tokens + p.block_tokens - 1) / p.block_tokens));
   const size_t smem = (size_t)p.block_tokens * p.half * sizeof(float2);
   if (wide) launch_pdl(rotary_kernel<T, true, PAGED>, grid, dim3(kRotaryThreads), smem, ctx->stream, p);
