@@ -11,7 +11,7 @@ CSRC = os.path.join(ROOT, "turbotransformers_b200", "csrc")
 
 
 class Split(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int) for n in ("block_heads", "blocks", "head_blocks", "tile_tokens", "unit_shift", "causal")]
+    _fields_ = [(n, ctypes.c_int) for n in ("block_heads", "blocks", "head_blocks", "tile_tokens", "unit_shift", "causal", "half", "pair_shift")]
 
 
 class Place(ctypes.Structure):
@@ -24,7 +24,7 @@ def rules(tmp_path_factory):
     src, so = d / "rules.cpp", d / "rules.so"
     src.write_text('#include "ttb_paged_rules.cuh"\nusing namespace ttb::paged;\nextern "C" {\n'
                    'int64_t floor_sum_(int64_t n, int64_t m, int64_t a, int64_t b) { return floor_sum(n, m, a, b); }\n'
-                   'void split_(int heads, int kv, int rows, int parts, int unit, int causal, Split* s) { *s = split_of(heads, kv, rows, parts, unit, causal); }\n'
+                   'void split_(int heads, int kv, int rows, int parts, int unit, int causal, int pair, Split* s) { *s = split_of(heads, kv, rows, parts, unit, causal, pair); }\n'
                    'int64_t units_of_sequence_(const Split* s, int64_t past, int64_t n) { return units_of_sequence(*s, past, n); }\n'
                    'int64_t units_of_tile_(const Split* s, int64_t past, int64_t n, int64_t t) { return units_of_tile(*s, past, n, t); }\n'
                    'void place_(const Split* s, int64_t past, int64_t n, int64_t x, Place* p) { *p = place_of(*s, past, n, x); }\n'
@@ -34,7 +34,7 @@ def rules(tmp_path_factory):
     lib = ctypes.CDLL(str(so))
     i64 = ctypes.c_int64
     lib.floor_sum_.restype, lib.floor_sum_.argtypes = i64, [i64] * 4
-    lib.split_.argtypes = [ctypes.c_int] * 6 + [ctypes.POINTER(Split)]
+    lib.split_.argtypes = [ctypes.c_int] * 7 + [ctypes.POINTER(Split)]
     lib.units_of_sequence_.restype, lib.units_of_sequence_.argtypes = i64, [ctypes.POINTER(Split), i64, i64]
     lib.units_of_tile_.restype, lib.units_of_tile_.argtypes = i64, [ctypes.POINTER(Split), i64, i64, i64]
     lib.place_.argtypes = [ctypes.POINTER(Split), i64, i64, i64, ctypes.POINTER(Place)]
@@ -55,7 +55,7 @@ def test_lattice_points_under_a_line(rules):
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (12, 12), (32, 8), (7, 1), (40, 2), (20, 1), (300, 1), (64, 1)])
 def test_a_tile_holds_whole_tokens_and_every_head_once(rules, heads, kv_heads, rows, parts):
     s = Split()
-    rules.split_(heads, kv_heads, rows, parts, 128, 1, s)
+    rules.split_(heads, kv_heads, rows, parts, 128, 1, 0, s)
     group = heads // kv_heads
     assert s.tile_tokens >= 1 and s.tile_tokens % parts == 0 and s.tile_tokens // parts * s.block_heads <= rows
     taken = [(b // s.head_blocks, h) for b in range(s.blocks) for h in range(b % s.head_blocks * s.block_heads, min(group, (b % s.head_blocks + 1) * s.block_heads))]
@@ -63,17 +63,20 @@ def test_a_tile_holds_whole_tokens_and_every_head_once(rules, heads, kv_heads, r
     assert all(b % s.head_blocks * s.block_heads < group for b in range(s.blocks))
 
 
+@pytest.mark.parametrize("pair", [0, 1])
 @pytest.mark.parametrize("causal", [0, 1])
 @pytest.mark.parametrize("heads,kv_heads,rows,parts,unit", [(12, 12, 16, 1, 128), (32, 8, 16, 1, 128), (7, 1, 128, 2, 128), (6, 2, 128, 2, 64), (40, 1, 16, 1, 128)])
-def test_every_unit_has_its_place(rules, heads, kv_heads, rows, parts, unit, causal):
+def test_every_unit_has_its_place(rules, heads, kv_heads, rows, parts, unit, causal, pair):
     s, p, rng = Split(), Place(), random.Random(heads * rows + causal)
-    rules.split_(heads, kv_heads, rows, parts, unit, causal, s)
+    rules.split_(heads, kv_heads, rows, parts, unit, causal, pair, s)
     for past, n in [(0, 0), (0, 1), (unit - 1, 1), (unit, 1), (0, unit + 1), (1000, 3)] + [(rng.randint(0, 700), rng.randint(1, 400)) for _ in range(12)]:
         tiles = -(-n // s.tile_tokens)
         line = []
         for t in range(tiles):
             keys = past + (min(n, (t + 1) * s.tile_tokens) if causal else n)
             units = -(-keys // unit)
+            if parts == 2 and n - t * s.tile_tokens <= s.tile_tokens // 2:  # one set's rows: both sets take its units in turn
+                units = -(-units // (1 + pair))
             assert rules.units_of_tile_(s, past, n, t) == units
             line += [(t, b, units, u) for b in range(s.blocks) for u in range(units)]
         assert rules.units_of_sequence_(s, past, n) == len(line)

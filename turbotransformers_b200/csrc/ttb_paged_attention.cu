@@ -563,10 +563,13 @@ int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, P
     j.parts[n] = p.parts;
     j.rows[n++] = rows[i];
     if (i == 0) {
-      p.split = split_of((int)heads, (int)kv->kv_heads, rows[0], 1, kUnit, p.split.causal);
+      p.split = split_of((int)heads, (int)kv->kv_heads, rows[0], 1, kUnit, p.split.causal, 0);
       st = groups == 1 ? launch_rows<T, D, 1>(ctx, kv, heads, p) : groups == 2 ? launch_rows<T, D, 2>(ctx, kv, heads, p) : launch_rows<T, D, 4>(ctx, kv, heads, p);
     } else {
-      p.split = split_of((int)heads, (int)kv->kv_heads, kManyRows / 2, 2, kUnit, p.split.causal);
+      // A tile of one set's rows takes two units of keys in the time of one of both sets' with heads of 64 (six prompts of 200 to 2000 tokens: 130 us, 135 with each
+      // counted as one). With heads of 128 it waits for values, whose ring is two tiles long, and a unit takes more than half (a chunk of 4000 tokens over
+      // 12000: 1040 us in pairs, 900 alone).
+      p.split = split_of((int)heads, (int)kv->kv_heads, kManyRows / 2, 2, kUnit, p.split.causal, D == 64 ? 1 : 0);
       st = paged_tc_launch(ctx, dtype, kv, heads, p);
     }
   }

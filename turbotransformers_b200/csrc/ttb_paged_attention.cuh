@@ -189,9 +189,11 @@ constexpr int kRingWorks = 8;
 
 __device__ __forceinline__ Work work_of(const Params& p, const Part& t, int slot) {
   Work w;
-  w.units = max(0, min(t.take, (t.keys + kUnit - 1) / kUnit - (int)t.first));
-  w.turns = w.count[0] = w.count[1] = 0;
-  w.first = (int)t.first;
+  w.turns = t.rows <= p.split.half * p.split.block_heads;
+  const int shift = w.turns ? p.split.pair_shift : 0;
+  w.first = (int)t.first << shift;
+  w.units = max(0, min(t.take << shift, (t.keys + kUnit - 1) / kUnit - w.first));
+  w.count[0] = w.count[1] = 0;
   w.b = t.b;
   w.key_row = t.block / p.split.head_blocks << p.s.page_shift;
   w.keys = t.keys;

@@ -87,8 +87,7 @@ __device__ __forceinline__ float hi2(unsigned long long s) { return __uint_as_fl
 
 // How a part's units fall to the two sets.
 __device__ __forceinline__ void share_out(const Params& p, Work* w) {
-  const int tokens = p.split.tile_tokens / 2;  // of a set
-  w->turns = w->rows <= tokens * p.split.block_heads;
+  const int tokens = p.split.half;  // of a set
   if (w->turns) {
     w->count[0] = (w->units + 1) / 2;
     w->count[1] = w->units / 2;
@@ -159,7 +158,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const int ctas = ctas_of(total, (int)gridDim.x, 1), cta = blockIdx.x;
   const long long lo = cta < ctas ? first_unit(total, ctas, cta) : 0, hi = cta < ctas ? first_unit(total, ctas, cta + 1) : 0;
   if (cta >= ctas && threadIdx.x == 0) p.parts.cuts[cta].pieces = 0;
-  const int set_tokens = p.split.tile_tokens / 2;
+  const int set_tokens = p.split.half;
   Work* works = reinterpret_cast<Work*>(smem + S::kWorks);
   // The n-th part, for every warp but the one that works them out. False: no part, there are no more or something gave up.
   auto take_part = [&](uint32_t n, Work* w) {

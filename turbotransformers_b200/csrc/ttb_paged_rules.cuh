@@ -78,10 +78,12 @@ struct Split {
   int blocks;       // head blocks of a sequence, over all key heads
   int head_blocks;  // of them a key head's
   int tile_tokens, unit_shift, causal;
+  int half;         // of two sets: tokens of one. A tile of no more is both sets' together, which take its units of keys in turn:
+  int pair_shift;   // so many of them (log2) are one unit of the line
 };
 
 // `rows` rows a tile of `parts` separate sets: a set's rows are whole tokens. `unit` is a power of two.
-TTB_PAGED_FN Split split_of(int heads, int kv_heads, int rows, int parts, int unit, int causal) {
+TTB_PAGED_FN Split split_of(int heads, int kv_heads, int rows, int parts, int unit, int causal, int pair_shift) {
   Split s;
   const int group = heads / kv_heads;
   s.head_blocks = (group + rows - 1) / rows;
@@ -89,6 +91,8 @@ TTB_PAGED_FN Split split_of(int heads, int kv_heads, int rows, int parts, int un
   s.head_blocks = (group + s.block_heads - 1) / s.block_heads;  // (none of them empty)
   s.blocks = kv_heads * s.head_blocks;
   s.tile_tokens = rows / s.block_heads * parts;
+  s.half = parts == 2 ? s.tile_tokens / 2 : 0;
+  s.pair_shift = pair_shift;
   s.unit_shift = 0;
   while ((1 << s.unit_shift) < unit) ++s.unit_shift;
   s.causal = causal;
@@ -105,18 +109,21 @@ TTB_PAGED_FN int64_t units_of(const Split& s, int64_t keys) { return (keys + (1 
 
 // of one head block of tile t: of the keys that its last token sees
 TTB_PAGED_FN int64_t units_of_tile(const Split& s, int64_t past, int64_t n, int64_t t) {
-  const int64_t end = (t + 1) * s.tile_tokens;
-  return units_of(s, past + (s.causal && end < n ? end : n));
+  const int64_t end = (t + 1) * s.tile_tokens, units = units_of(s, past + (s.causal && end < n ? end : n));
+  return n - t * s.tile_tokens <= s.half ? (units + (1 << s.pair_shift) - 1) >> s.pair_shift : units;
 }
 
 // of the tiles before t together (t at most tiles_of)
 TTB_PAGED_FN int64_t units_before_tile(const Split& s, int64_t past, int64_t n, int64_t t) {
   if (t == 0) return 0;
-  const int64_t all = units_of(s, past + n);
-  if (!s.causal || n <= s.tile_tokens) return t * all;
-  const int64_t whole = quotient(n, s.tile_tokens);  // tiles whose last token is not the sequence's
-  const int64_t m = t < whole ? t : whole;
-  return floor_sum(m, 1 << s.unit_shift, s.tile_tokens, past + s.tile_tokens + (1 << s.unit_shift) - 1) + (t > m ? all : 0);
+  const int64_t tiles = tiles_of(s, n);
+  int64_t last = 0;  // of the sequence's last tile, where it is among them
+  if (t == tiles) {
+    last = units_of_tile(s, past, n, --t);
+    if (t == 0) return last;
+  }
+  if (!s.causal) return t * units_of(s, past + n) + last;
+  return floor_sum(t, 1 << s.unit_shift, s.tile_tokens, past + s.tile_tokens + (1 << s.unit_shift) - 1) + last;
 }
 
 TTB_PAGED_FN int64_t units_of_sequence(const Split& s, int64_t past, int64_t n) { return n > 0 ? units_before_tile(s, past, n, tiles_of(s, n)) * s.blocks : 0; }
