@@ -68,7 +68,8 @@ def status():
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("T,heads,kv,d,dim,interleaved", [
     (1, 4, 2, 64, 64, False), (1, 1, 1, 8, 2, True), (5, 3, 1, 128, 128, True), (33, 12, 12, 64, 32, False), (700, 8, 2, 128, 64, True),
-    (3, 2, 2, 72, 20, False), (3, 2, 2, 72, 20, True), (2, 2, 1, 512, 512, False), (9, 5, 5, 96, 24, True), (9, 5, 5, 96, 48, False)])
+    (3, 2, 2, 72, 20, False), (3, 2, 2, 72, 20, True), (2, 2, 1, 512, 512, False), (9, 5, 5, 96, 24, True), (9, 5, 5, 96, 48, False),
+    (5001, 3, 2, 24, 16, False), (4800, 1, 0, 16, 16, False), (2500, 7, 1, 40, 6, True), (1300, 5, 3, 64, 64, False), (2, 2000, 1000, 128, 128, False)])
 def test_rotary(dt, T, heads, kv, d, dim, interleaved):
     g, dtype = gen(T + d + dim), DT[dt]
     q, k = randn(g, T, heads, d, dtype=dtype), randn(g, T, kv, d, dtype=dtype)
@@ -262,6 +263,50 @@ def test_attention(dt, page, past, new, heads, kv, d, causal):
     assert (out[sum(new):] == 5.0).all() and (out[:, heads] == 5.0).all()
     again = tt.paged_attention(q, *pool.args(), causal=causal, scale=0.2)
     assert torch.equal(again[:sum(new)], got[:sum(new)])  # the same on every run
+
+
+# No more tokens than sequences: tiles of 8, 16 and 32 rows, and heads that need more, for all of them; then one sequence of a tile's rows, or some more.
+STEPS = [
+    # page, past, new, heads, kv heads, head size, causal
+    (16, [0, 1, 127, 128, 700], [1, 1, 1, 1, 1], 5, 1, 64, True), (16, [40, 3000, 0], [1, 1, 1], 9, 1, 128, True), (32, [127, 0, 1300], [1, 1, 1], 32, 2, 64, True),
+    (16, [2000, 15, 16], [1, 1, 1], 16, 1, 128, False), (64, [129, 0, 5000], [1, 1, 1], 17, 1, 64, True), (16, [31, 6000], [1, 1], 64, 2, 128, True),
+    (16, [255, 10], [1, 1], 32, 1, 64, False), (16, [300, 0, 77], [1, 1, 1], 33, 1, 64, True), (16, [90, 5, 300, 0, 0, 2], [0, 6, 0, 0, 0, 0], 24, 2, 64, True),
+    (32, [90, 5, 300, 40], [1, 0, 3, 0], 40, 2, 128, True), (16, [10] * 40, [0] * 39 + [40], 4, 4, 64, True), (16, [7000], [7], 16, 1, 64, True), (16, [7000], [8], 32, 2, 64, False),
+    (256, [4000], [2], 32, 2, 128, True), (16, [1000], [4], 4, 2, 128, True), (128, [999], [9], 4, 4, 64, True),
+]
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("page,past,new,heads,kv,d,causal", STEPS)
+def test_attention_of_a_step(dt, page, past, new, heads, kv, d, causal):
+    dtype = DT[dt]
+    pool = Pool(sum(past) + heads, dtype, past, new, kv, d, page)
+    pool.fill_new(dtype, kv, d)
+    q = randn(pool.g, sum(new), heads, d, dtype=dtype)
+    got = tt.paged_attention(q, *pool.args(), causal=causal, scale=0.2)
+    assert status() == _capi.OK
+    want, off = attended(q, pool, causal, 0.2)
+    far = (got.double() - want).abs()
+    assert (far <= off).all(), f"{(far / off).max().item():.3g} times the tolerance"
+    assert torch.equal(tt.paged_attention(q, *pool.args(), causal=causal, scale=0.2), got)
+
+
+@pytest.mark.parametrize("heads", [8, 16, 32])
+def test_attention_of_a_step_with_scores_far_apart(heads):
+    """As below, for tiles of each number of rows, every row with a course of its own."""
+    past, d = 1500, 64
+    pool = Pool(4, torch.float16, [past, past], [1, 1], 1, d, 16)
+    pool.fill_new(torch.float16, 1, d)
+    for b in range(2):
+        for j in range(past + 1):
+            page, slot = pool.rows[b][j // 16], j % 16
+            pool.keys[page, :, slot] = pool.keys[page, :, slot] * 0.01 + (j % 700) / 64.0 * (1 if j < 1100 else 0.3)
+    q = torch.ones(2, heads, d, dtype=torch.float16, device=DEV) + randn(pool.g, 2, heads, d, dtype=torch.float16) * 0.01
+    q *= (1 - torch.arange(heads, device=DEV) % 3 * 0.75)[:, None].half()  # rising, rising slowly, falling
+    got = tt.paged_attention(q, *pool.args(), scale=1.0)
+    want, off = attended(q, pool, True, 1.0)
+    # scores of up to 700: their fp32 sums are off by 64 roundings of up to 700 * 2^-24 at most, 2^-9 in the exponent
+    assert ((got.double() - want).abs() <= off + 2.0 ** -8 * want.abs().amax()).all()
 
 
 @pytest.mark.parametrize("new", [1, 200])
