@@ -1,11 +1,17 @@
 // Attention of the new tokens of ragged sequences over a pool of cache pages: out = softmax(scale * q . K^T) . V, token i of a sequence over the cached
 // tokens 0 .. past + i (causal), or over all of them. `group` query heads share a key head.
 //
-// For few rows the call is bound by reading the keys and values once. All query rows of a tile (tokens x heads of one key head, up to 16) go through the keys
+// For few rows the call is bound by reading the keys and values once. All query rows of a tile (tokens x heads of one key head, 8, 16 or 32) go through the keys
 // together; the line of all tiles' keys is dealt out to one CTA an SM in equal stretches (ttb_paged_rules.cuh), so that one long sequence and a ragged batch
-// keep every SM's loads busy alike. In a CTA one warp loads (units of 128 tokens, TMA boxes of a page, 128-byte swizzled, 192 KB on their way) and runs on
-// into the next tile; four warps take 32 keys each of every unit, with a softmax state of their own (running maximum and sum in fp32, mma.sync m16n8k16), and join
-// the four states at the tile's end. Parts of a tile that was cut go to a workspace in fp32 and a second kernel joins them, in the order of the keys.
+// keep every SM's loads busy alike. In a CTA four warps load (units of 128 tokens, TMA boxes of a page, 128-byte swizzled, 192 KB on their way) and run on
+// into the next tile; four take 32 keys each of every unit, with a softmax state of their own, and join the four states at the tile's end. Their products are
+// mma.sync m16n8k16 with the keys as rows: a tile of eight queries fills it, where the tensor memory's 128 rows would be empty but for eight. Parts of a tile that was cut
+// go to a workspace in fp32 and a second kernel joins them, in the order of the keys.
+// A row's reference is the maximum of its first keys, raised (and its sums rescaled) only where the probabilities of 32 keys sum to more than 2^15; the division by the sum
+// makes the result independent of it. Scores, references and sums are fp32; the probabilities are rounded to the values' 16 bits, the only form in which the
+// tensor cores take both (half a step of each, of both signs, against a sum of them that is not rounded).
+// 64 requests of 20 to 4000 tokens, 12 heads of 64, fp16: 89 us, 5.1 TB/s (110 with one loading warp and 16-row tiles throughout). One token over 8000, 32 heads of
+// 128 on 8 key heads, bf16: 17 us, of which some 7 are the join and its launch.
 #include <algorithm>
 #include <climits>
 #include <cmath>

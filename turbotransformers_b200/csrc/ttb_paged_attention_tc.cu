@@ -10,7 +10,12 @@
 //                 the order QK(0), PV(0), QK(1), PV(1), ...; everything a product waits for but the softmax is a barrier poll
 //   warps 4..11 : softmax, a warpgroup a set, a row a thread: scores from TMEM, exp2 with the scale folded in, P back to TMEM in 16 bits. The row's reference is the maximum of
 //                 its first tile; it is raised (and O rescaled) only where the sum of 32 probabilities passes 2^15: the division by the sum makes the result independent of it.
-// A tile's output is written while the next one's first scores are made. Every wait is bounded.
+// A tile's output is written while the next one's first scores are made. Every wait is bounded. The probabilities are rounded to the values' 16 bits, as in the kernel for few
+// rows; their sums are not.
+// 4000 tokens over 12000, 32 heads of 128 on 8 key heads, bf16: 900 us, 1.02 PFLOP/s of products that the mask leaves; a pair of units takes 4400 cycles, of which the products
+// are 2050 and a set's exponentials alone 1024 on their own unit, with the conversions, sums and tensor memory traffic of 256 rows beside them. 16 requests of 3 to 6
+// tokens over up to 16000, 64 heads of 128 on 8: 155 us, 4.1 TB/s: two tiles of values are the most that fit beside the queries, and their way from memory shows
+// (a third place for keys changed nothing).
 #include <algorithm>
 #include <type_traits>
 
