@@ -537,7 +537,7 @@ template <typename T, int D>
 int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, Params& p) {
   // Which kernels, and the rows of a tile of the one for few. The host knows the sum of the new tokens only. With no more tokens than sequences, tiles of a token's rows (up to 32)
   // take all of them, a sequence of several tokens several tiles. Otherwise tiles of an average sequence's rows, 16 at most, and the sequences that have more go
-  // to the kernel for many (16 requests of 3 to 6 tokens, 8 heads to a key head, over up to 16000: 143 us there, 171 with those of 32 rows in this one).
+  // to the kernel for many (16 requests of 3 to 6 tokens, 8 heads to a key head, over up to 16000: 153 us there, 171 with those of 32 rows in this one).
   const int64_t tokens = p.s.tokens, B = kv->B, each = (tokens + B - 1) / B * p.group;
   const int64_t need = std::max<int64_t>(p.group, std::min<int64_t>(each, 16));
   const int groups = need <= 8 ? 1 : need <= 16 ? 2 : 4, few = 8 * groups / p.group;
@@ -572,7 +572,7 @@ int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, P
       p.split = split_of((int)heads, (int)kv->kv_heads, rows[0], 1, kUnit, p.split.causal, 0);
       st = groups == 1 ? launch_rows<T, D, 1>(ctx, kv, heads, p) : groups == 2 ? launch_rows<T, D, 2>(ctx, kv, heads, p) : launch_rows<T, D, 4>(ctx, kv, heads, p);
     } else {
-      // A tile of one set's rows takes two units of keys in the time of one of both sets' with heads of 64 (six prompts of 200 to 2000 tokens: 130 us, 135 with each
+      // A tile of one set's rows takes two units of keys in the time of one of both sets' with heads of 64 (six prompts of 200 to 2000 tokens: 130 us, and 135 with each
       // counted as one). With heads of 128 it waits for values, whose ring is two tiles long, and a unit takes more than half (a chunk of 4000 tokens over
       // 12000: 1040 us in pairs, 900 alone).
       p.split = split_of((int)heads, (int)kv->kv_heads, kManyRows / 2, 2, kUnit, p.split.causal, D == 64 ? 1 : 0);

@@ -9,12 +9,12 @@
 //   warps 1, 3  : matrix products of a set each - S = Q K^T (128 x 128, fp32 in TMEM), O += P V with P in TMEM over the scores it came from, V as it lies, in
 //                 the order QK(0), PV(0), QK(1), PV(1), ...; everything a product waits for but the softmax is a barrier poll
 //   warps 4..11 : softmax, a warpgroup a set, a row a thread: scores from TMEM, exp2 with the scale folded in, P back to TMEM in 16 bits. The row's reference is the maximum of
-//                 its first tile; it is raised (and O rescaled) only where the sum of 32 probabilities passes 2^15: the division by the sum makes the result independent of it.
+//                 its first 32 keys; it is raised (and O rescaled) only where the sum of 32 probabilities passes 2^15: the division by the sum makes the result independent of it.
 // A tile's output is written while the next one's first scores are made. Every wait is bounded. The probabilities are rounded to the values' 16 bits, as in the kernel for few
 // rows; their sums are not.
 // 4000 tokens over 12000, 32 heads of 128 on 8 key heads, bf16: 900 us, 1.02 PFLOP/s of products that the mask leaves; a pair of units takes 4400 cycles, of which the products
 // are 2050 and a set's exponentials alone 1024 on their own unit, with the conversions, sums and tensor memory traffic of 256 rows beside them. 16 requests of 3 to 6
-// tokens over up to 16000, 64 heads of 128 on 8: 155 us, 4.1 TB/s: two tiles of values are the most that fit beside the queries, and their way from memory shows
+// tokens over up to 16000, 64 heads of 128 on 8: 153 us, 4.1 TB/s: two tiles of values are the most that fit beside the queries, and their way from memory shows
 // (a third place for keys changed nothing).
 #include <algorithm>
 #include <type_traits>
@@ -520,30 +520,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const bool edge = k0 + kUnit > all_see;
           uint32_t r[32];
           auto mask = [&](int c) {
-            if (edge) {
+            if (k0 + (c + 1) * 32 > all_see) {
               const int n = limit - k0 - c * 32;
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (e >= n) r[e] = 0xff800000u;
             }
           };
+          // The reference: any score near the largest does, and another pass over the tile would cost a third of its softmax (six prompts of 200 to 2000 tokens, heads of
+          // 64: 130 us with the maximum of all 128, 125). A row that sees none of these 32 keys sees none of the others.
           if (j == 0) {
-#pragma unroll 1
-            for (int c = 0; c < live; ++c) {
-              tmem_ld32_issue(ts + (uint32_t)(c * 32), r);
-              tmem_ld_wait();
-              mask(c);
-              float top = -INFINITY;
+            tmem_ld32_issue(ts, r);
+            tmem_ld_wait();
+            mask(0);
+            float top = -INFINITY;
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) top = fmaxf(fmaxf(top, __uint_as_float(r[e])), __uint_as_float(r[e + 1]));
-              m_used = fmaxf(m_used, top * p.scale);
-            }
+            for (int e = 0; e < 32; e += 2) top = fmaxf(fmaxf(top, __uint_as_float(r[e])), __uint_as_float(r[e + 1]));
+            m_used = top * p.scale;
           }
-          // A tile that every row sees the whole of, against a reference that an earlier one gave: straight through, P kept until its sum says that the reference still
-          // holds. Short code, since the instruction cache is the other warps' too (with masks and rescaling in it 16 products took 3500 cycles in place of 1250).
+          // A tile that every row sees the whole of: straight through, P kept until its sum says that the reference still holds. Short code, since the instruction cache is the other warps' too (with masks and rescaling in it 16 products took 3500 cycles in place of 1250).
           float l0 = 0.f, l1 = 0.f;
           bool done = false;
-          if (j > 0 && !edge) {
+          if (!edge) {
             uint32_t pk[2][32];
             unsigned long long sum = 0, sum2 = 0;
             const float m_sub = m_used == -INFINITY ? 0.f : m_used;
