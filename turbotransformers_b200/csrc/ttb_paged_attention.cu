@@ -454,7 +454,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if ((!ok || *abort_flag) && lane == 0) atomicExch(p.s.status, (int)TTB_ERR_DEVICE_WAIT);
 }
 
-// Joins the parts of the tiles that were cut, of both kernels: a block (and its neighbours along y) for each of their CTAs, a warp for each row, parts in the
+// Joins the parts of the tiles that were cut, of both kernels: a block (and its neighbours along y) for each of their CTAs, R rows a warp, parts in the
 // order of the keys.
 struct JoinParams {
   Parts parts[2];
@@ -462,7 +462,7 @@ struct JoinParams {
   void* out;
   long long ldo;
 };
-template <typename T, int D>
+template <typename T, int D, int R>
 __global__ void __launch_bounds__(128)
 paged_join_kernel(const JoinParams p) {
   pdl_trigger();
@@ -472,48 +472,75 @@ paged_join_kernel(const JoinParams p) {
   const int stride = which ? p.rows[1] : p.rows[0];
   const Cut c = parts.cuts[blockIdx.x];
   if (c.pieces == 0) return;
-  constexpr int V = D / 32;
-  for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < c.rows; row += gridDim.y * 4) {
-    const int i = row / c.block_heads, g = row % c.block_heads;
-    if (g >= c.heads) continue;
-    auto at = [&](int k) { return (long long)(k == 0 ? c.slot : 2 * ((int)blockIdx.x + k)) * stride + row; };
-    float M = -INFINITY;
-    for (int k = lane; k < c.pieces; k += 32) M = fmaxf(M, parts.ml[at(k)].x);
-    M = warp_max(M);
-    const float sub = M == -INFINITY ? 0.f : M;
-    float L = 0.f, o[V];
+  constexpr int V = D / 32, E = 8 / R;  // sums of eight rows and parts are on their way
+  auto slot = [&](int k) { return (long long)(k == 0 ? c.slot : 2 * ((int)blockIdx.x + k)) * stride; };
+  for (int row0 = (blockIdx.y * 4 + (threadIdx.x >> 5)) * R; row0 < c.rows; row0 += gridDim.y * 4 * R) {
+    float M[R], L[R], o[R][V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = 0.f;
-    for (int k0 = 0; k0 < c.pieces; k0 += 32) {  // a lane has a part's weight; the parts' sums come eight at a time
-      float mine = 0.f;
-      if (k0 + lane < c.pieces) {
-        const float2 ml = parts.ml[at(k0 + lane)];
-        mine = ex2(ml.x - sub);
-        L = fmaf(ml.y, mine, L);
+    for (int r = 0; r < R; ++r) {
+      M[r] = -INFINITY;
+      L[r] = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[r][v] = 0.f;
+    }
+    for (int k = lane; k < c.pieces; k += 32) {
+      const long long at = slot(k) + row0;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (row0 + r < c.rows) M[r] = fmaxf(M[r], parts.ml[at + r].x);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      M[r] = warp_max(M[r]);
+      M[r] = M[r] == -INFINITY ? 0.f : M[r];
+    }
+    for (int k0 = 0; k0 < c.pieces; k0 += 32) {  // a lane has a part's weights
+      float mine[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        mine[r] = 0.f;
+        if (k0 + lane < c.pieces && row0 + r < c.rows) {
+          const float2 ml = parts.ml[slot(k0 + lane) + row0 + r];
+          mine[r] = ex2(ml.x - M[r]);
+          L[r] = fmaf(ml.y, mine[r], L[r]);
+        }
       }
       const int n = min(32, c.pieces - k0);
-      for (int k1 = 0; k1 < n; k1 += 8) {
-        float x[8][V];
+      for (int k1 = 0; k1 < n; k1 += E) {
+        float x[E][R][V];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < E; ++e)
           if (k1 + e < n) {
+            const float* src = parts.o + (slot(k0 + k1 + e) + row0) * D + lane;
 #pragma unroll
-            for (int v = 0; v < V; ++v) x[e][v] = parts.o[at(k0 + k1 + e) * D + v * 32 + lane];
+            for (int r = 0; r < R; ++r)
+              if (row0 + r < c.rows) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[e][r][v] = src[r * D + v * 32];
+              }
           }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < E; ++e) {
           if (k1 + e >= n) break;
-          const float w = __shfl_sync(0xffffffffu, mine, k1 + e);  // zero for a part without a key for this row, which has no sums
 #pragma unroll
-          for (int v = 0; v < V; ++v) o[v] = w == 0.f ? o[v] : fmaf(x[e][v], w, o[v]);
+          for (int r = 0; r < R; ++r) {
+            const float w = __shfl_sync(0xffffffffu, mine[r], k1 + e);  // zero for a part without a key for this row, which has no sums
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[r][v] = w == 0.f ? o[r][v] : fmaf(x[e][r][v], w, o[r][v]);
+          }
         }
       }
     }
-    L = warp_sum(L);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    T* dst = static_cast<T*>(p.out) + (long long)(c.tok0 + i) * p.ldo + (long long)(c.head0 + g) * D;
 #pragma unroll
-    for (int v = 0; v < V; ++v) dst[v * 32 + lane] = from_f<T>(o[v] * inv);
+    for (int r = 0; r < R; ++r) {
+      const int row = row0 + r, i = row / c.block_heads, g = row % c.block_heads;
+      const float l = warp_sum(L[r]);
+      if (row >= c.rows || g >= c.heads) continue;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* dst = static_cast<T*>(p.out) + (long long)(c.tok0 + i) * p.ldo + (long long)(c.head0 + g) * D;
+#pragma unroll
+      for (int v = 0; v < V; ++v) dst[v * 32 + lane] = from_f<T>(o[r][v] * inv);
+    }
   }
 }
 
@@ -580,7 +607,8 @@ int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, P
     }
   }
   if (!st) {
-    launch_pdl(paged_join_kernel<T, D>, dim3((unsigned)ctas, used[1] ? 16 : rows[0] / 4, (unsigned)n), dim3(128), 0, ctx->stream, j);
+    if (used[1]) launch_pdl(paged_join_kernel<T, D, 4>, dim3((unsigned)ctas, kManyRows / 16, (unsigned)n), dim3(128), 0, ctx->stream, j);
+    else launch_pdl(paged_join_kernel<T, D, 1>, dim3((unsigned)ctas, rows[0] / 4, (unsigned)n), dim3(128), 0, ctx->stream, j);
     st = launched(ctx, "paged_attention_join");
   }
   const int f = ttb_free(ctx, ws, "paged_attention/parts");
