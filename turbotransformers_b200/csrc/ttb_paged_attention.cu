@@ -11,7 +11,7 @@
 // makes the result independent of it. Scores, references and sums are fp32; the probabilities are rounded to the values' 16 bits, the only form in which the
 // tensor cores take both (half a step of each, of both signs, against a sum of them that is not rounded).
 // 64 requests of 20 to 4000 tokens, 12 heads of 64, fp16: 89 us, 5.1 TB/s (110 with one loading warp and 16-row tiles throughout). One token over 8000, 32 heads of
-// 128 on 8 key heads, bf16: 17 us, of which some 7 are the join and its launch.
+// 128 on 8 key heads, bf16: 15 us, of which 3 go by before the first load (the sequences, the part, its pages) and some 5 are the join and its launch.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -148,7 +148,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 
   if (warp >= kWarps) {
     // ---- loads: a lane for each box (a page, or 128 keys) of keys or values and half of a head, every fourth of them a warp's: a copy takes its thread some 60
-    // cycles to issue, one lane after the other. The pages of a unit are looked up while the one before is loaded. The first of the warps works the parts out.
+    // cycles to issue, one lane after the other. A lane's pages are looked up two units ahead. The first of the warps works the parts out.
     const int loader = warp - kWarps;
     const int page_tokens = 1 << p.s.page_shift, box_rows = min(page_tokens, kUnit);
     const int at = lane * kLoaders + loader, box = at / (2 * S::kHalves), which = at / S::kHalves & 1, half = at % S::kHalves;
@@ -179,18 +179,19 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int key = (w.first + i) * kUnit + box * box_rows;
       return key < w.keys && box * box_rows < kUnit ? p.s.table[w.b * p.s.table_stride + (key >> p.s.page_shift)] : 0;
     };
-    Work w = {}, w2;
-    int page = 0;
-    for (;; ++n) {  // w2 is the n-th part; the loads are those of w, the one before
-      const bool more = loader == 0 ? publish(&w2) : take_part(n, &w2);
-      if (w.units == 0 && more) page = page_at(w2, 0);  // at the beginning, and behind a part without keys (more tokens than the table lists)
-      if (n > 0 && loader == 0 && ok) {
-        ok = __all_sync(0xffffffffu, mbar_wait(q_empty(n - 1), q_phase(n - 1) ^ 1u, abort_flag));
+    auto next = [&](Work* w) { return loader == 0 ? publish(w) : take_part(n, w); };  // the n-th part
+    Work w, w2;
+    bool more = next(&w);
+    int page = more ? page_at(w, 0) : 0, page2 = more ? page_at(w, 1) : 0;  // the lane's, of this unit and the next
+    while (more) {
+      if (loader == 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(q_empty(n), q_phase(n) ^ 1u, abort_flag));
         if (ok && lane == 0) {
-          mbar_expect_tx(q_full(n - 1), (uint32_t)(p.split.tile_tokens * p.split.block_heads * D * 2));
-          for (int h = 0; h < S::kHalves; ++h) tma_load_3d(q_at(n - 1) + h * S::kQHalf, &tm_q, q_full(n - 1), h * 64, w.head0, w.tok0);
+          mbar_expect_tx(q_full(n), (uint32_t)(p.split.tile_tokens * p.split.block_heads * D * 2));
+          for (int h = 0; h < S::kHalves; ++h) tma_load_3d(q_at(n) + h * S::kQHalf, &tm_q, q_full(n), h * 64, w.head0, w.tok0);
         }
       }
+      ++n;
       for (int i = 0; i < w.units && ok; ++i, ++g) {
         const int key = (w.first + i) * kUnit + box * box_rows;
         int mine = -1;
@@ -201,7 +202,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             mine = 0;
           }
         }
-        page = i + 1 < w.units ? page_at(w, i + 1) : more ? page_at(w2, 0) : 0;
         ok = __all_sync(0xffffffffu, mbar_wait(empty(g), phase(g) ^ 1u, abort_flag));
         if (!ok) break;
         const int boxes = __popc(__ballot_sync(0xffffffffu, mine >= 0));
@@ -210,8 +210,16 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (mine >= 0)
           tma_load_3d(keys_at(g) + which * S::kTile + half * S::kHalfBytes + box * box_rows * 128, which ? &tm_v : &tm_k, full(g), half * 64,
                       w.key_row + (key & (page_tokens - 1)), mine);
+        if (i == 0) more = next(&w2);
+        page = i + 1 < w.units ? page2 : more ? page_at(w2, 0) : 0;
+        page2 = i + 2 < w.units ? page_at(w, i + 2) : more ? page_at(w2, i + 2 - w.units) : 0;
       }
-      if (!more || !ok) break;
+      if (!ok) break;
+      if (w.units == 0) {  // a part without keys (more tokens than the table lists)
+        more = next(&w2);
+        page = more ? page_at(w2, 0) : 0;
+        page2 = more ? page_at(w2, 1) : 0;
+      }
       w = w2;
     }
     if (loader == 0 && !cut_here && lane == 0) p.parts.cuts[cta].pieces = 0;

@@ -66,18 +66,16 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v)
 __device__ __forceinline__ long long line_up(const Params& p, long long* prefix, long long* scratch, int threads) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   bool any_bad = false;
-  for (int b = tid; b < p.s.B; b += threads) {
-    bool bad;
-    const Sequence q = taken(p, b, &bad);
-    any_bad |= bad;
-    prefix[b] = units_of_sequence(p.split, q.past, q.n);
-  }
-  if (any_bad && blockIdx.x == 0) bad_index(p.s.status);
-  __syncthreads();
   long long carry = 0;
   for (int b0 = 0; b0 < p.s.B; b0 += threads) {
     const int b = b0 + tid;
-    const long long mine = b < p.s.B ? prefix[b] : 0;
+    long long mine = 0;
+    if (b < p.s.B) {
+      bool bad;
+      const Sequence q = taken(p, b, &bad);
+      any_bad |= bad;
+      mine = units_of_sequence(p.split, q.past, q.n);
+    }
     long long incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -92,8 +90,9 @@ __device__ __forceinline__ long long line_up(const Params& p, long long* prefix,
       carry += scratch[w];
     }
     if (b < p.s.B) prefix[b] = before + incl - mine;
-    __syncthreads();
+    if (b0 + threads < p.s.B) __syncthreads();  // the scratch's last readers are through
   }
+  if (any_bad && blockIdx.x == 0) bad_index(p.s.status);
   if (tid == 0) prefix[p.s.B] = carry;
   __syncthreads();
   return carry;
@@ -166,9 +165,9 @@ __device__ __forceinline__ int heads_of(const Params& p, int block) {
 
 // Whoever has the beginning of a tile that ends in another CTA's stretch, at unit u of the line, says so.
 __device__ __forceinline__ Cut cut_of(const Params& p, const Part& t, long long u, long long total, int cta, int ctas, int slot) {
-  int pieces = 1;
-#pragma unroll 1
-  while (cta + pieces < ctas && first_unit(total, ctas, cta + pieces) < u + t.units) ++pieces;
+  // CTA c begins before the tile's end if total * c / ctas, rounded down or not, is less than that
+  const int last = (int)quotient((u + t.units) * ctas + total - 1, total);
+  const int pieces = min(last, ctas) - cta;
   return Cut{pieces, slot, t.tok0, first_head(p, t.block), t.rows, p.split.block_heads, heads_of(p, t.block)};
 }
 
