@@ -69,7 +69,8 @@ def status():
 @pytest.mark.parametrize("T,heads,kv,d,dim,interleaved", [
     (1, 4, 2, 64, 64, False), (1, 1, 1, 8, 2, True), (5, 3, 1, 128, 128, True), (33, 12, 12, 64, 32, False), (700, 8, 2, 128, 64, True),
     (3, 2, 2, 72, 20, False), (3, 2, 2, 72, 20, True), (2, 2, 1, 512, 512, False), (9, 5, 5, 96, 24, True), (9, 5, 5, 96, 48, False),
-    (5001, 3, 2, 24, 16, False), (4800, 1, 0, 16, 16, False), (2500, 7, 1, 40, 6, True), (1300, 5, 3, 64, 64, False), (2, 2000, 1000, 128, 128, False)])
+    (5001, 3, 2, 24, 16, False), (4800, 1, 0, 16, 16, False), (2500, 7, 1, 40, 6, True), (1300, 5, 3, 64, 64, False), (2, 2000, 1000, 128, 128, False),
+    (7203, 21, 11, 64, 32, True), (7301, 30, 2, 128, 128, False), (8001, 2, 126, 32, 32, False), (7600, 33, 0, 64, 64, True)])
 def test_rotary(dt, T, heads, kv, d, dim, interleaved):
     g, dtype = gen(T + d + dim), DT[dt]
     q, k = randn(g, T, heads, d, dtype=dtype), randn(g, T, kv, d, dtype=dtype)
@@ -196,7 +197,8 @@ def attended(q, pool, causal, scale):
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("page,past,new,heads,kv,d,dim,interleaved,together", [
     (16, [0], [1], 4, 2, 64, 64, False, False), (16, [15, 16, 0, 31], [1, 1, 0, 2], 4, 1, 128, 64, True, False), (64, [0, 100], [130, 65], 6, 6, 64, 64, False, True),
-    (256, [255, 1], [3, 300], 8, 2, 128, 128, True, False), (32, [7] * 200, [1] * 200, 2, 2, 64, 16, False, True), (128, [0, 0, 5], [0, 7, 0], 3, 3, 64, 20, True, False)])
+    (256, [255, 1], [3, 300], 8, 2, 128, 128, True, False), (32, [7] * 200, [1] * 200, 2, 2, 64, 16, False, True), (128, [0, 0, 5], [0, 7, 0], 3, 3, 64, 20, True, False),
+    (64, [0, 100, 5], [3000, 4300, 1], 16, 8, 64, 32, True, False), (16, [7, 0, 0, 130], [1500, 0, 4000, 1800], 15, 9, 128, 128, False, True)])
 def test_append(dt, page, past, new, heads, kv, d, dim, interleaved, together):
     dtype = DT[dt]
     pool = Pool(sum(new) + page, dtype, past, new, kv, d, page, together)

@@ -15,9 +15,9 @@ namespace {
 // memory. The angle is a product of doubles in turns, of which the whole ones are dropped before it is rounded to fp32: a position of a
 // million times a frequency in fp32 would be off by a tenth of a radian. With a pool of pages, k is turned on its way into its page and v copied beside it: a pass
 // of its own over both, and a launch, saved. The rows are on their way while the block looks up its positions and pages.
-// 15000 tokens of 32 heads of 64, fp16, half of each turned: 27 us, 4.6 TB/s; 7900 tokens of prompts, 32 heads of 128 turned and 8 filed with their values: 42 us, 4.6 TB/s.
-// Units of a thread, threads of an SM and units of a block were measured together: two, 1536 and 1024 (four units and 1024 threads 31 and 47 us with the
-// launch for the first two, 31 and 51; one unit and 512 to a block 31 to 43, 49 to 63).
+// 8000 tokens of 40 heads of 128, fp32, all of each turned: 59 us, 5.5 TB/s; 64 and 200 tokens of 40 heads of 128, 16 bits: 5 and 7 us, a chain of dependent reads.
+// Units of a thread, threads of an SM and units of a block were measured together: two, 1536 and 1024 (15000 tokens of 32 heads of 64, fp16, and 7900 of 48 of 128, with the launch: 31 and 47 us;
+// four units and 1024 threads 31 and 51; one unit and 512 to a block 31 to 43 and 49 to 63).
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryTokens = 8;  // of a block, at most
 constexpr int kRotaryUnits = 2;   // that a thread has on their way
@@ -133,34 +133,10 @@ __device__ __forceinline__ void turn(Piece<T, false>& x, Piece<T, false>& y, boo
   y.w = from_f<T>(g * cs->x + f * cs->y);
 }
 
-template <typename T, bool WIDE, bool PAGED>
-__global__ void __launch_bounds__(kRotaryThreads, sizeof(T) == 2 ? 6 : 4)
-rotary_kernel(const RotaryParams p) {
-  extern __shared__ __align__(16) float2 cs[];  // [block_tokens][half]
-  __shared__ double s_pos[kRotaryTokens];
-  __shared__ long long s_page[kRotaryTokens];  // PAGED: the token's first element of the pools, -1: it has no place
-  pdl_trigger();
-  pdl_wait();
+// The block's positions, and (PAGED) the places of its tokens; then cosines and sines of all their pairs, times the scale. All threads.
+template <bool PAGED>
+__device__ __forceinline__ void block_angles(const RotaryParams& p, int t0, int n, double* s_pos, long long* s_page, float2* cs) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int t0 = blockIdx.x * p.block_tokens, n = min(p.block_tokens, p.tokens - t0);
-  const int units = n * p.rows * (int)p.per;
-  Piece<T, WIDE> x[kRotaryUnits], y[kRotaryUnits];
-  auto load = [&](int idx0) {
-#pragma unroll
-    for (int b = 0; b < kRotaryUnits; ++b) {
-      const int idx = idx0 + b * kRotaryThreads;
-      if (idx >= units) break;
-      const UnitPlace w = unit_place<WIDE>(p, idx);
-      const long long t = t0 + w.token;
-      const T* src;
-      if (w.head < p.heads) src = static_cast<const T*>(p.q) + t * p.ldq + w.head * p.d;
-      else if (!PAGED || w.head < p.heads + p.kv_heads) src = static_cast<const T*>(p.k) + t * p.ldk + (w.head - p.heads) * p.d;
-      else src = static_cast<const T*>(p.v) + t * p.ldv + (w.head - p.heads - p.kv_heads) * p.d;
-      x[b].load(src + w.first);
-      if (w.second >= 0) y[b].load(src + w.second);
-    }
-  };
-  load(tid);  // on their way while the block works out its positions
   for (int i = PAGED ? warp : tid; i < n; i += PAGED ? kRotaryThreads / 32 : kRotaryThreads) {
     const int t = t0 + i;
     if (!PAGED) {
@@ -196,7 +172,37 @@ rotary_kernel(const RotaryParams p) {
     cs[i] = make_float2(c * p.scale, s * p.scale);
   }
   __syncthreads();
+}
 
+template <typename T, bool WIDE, bool PAGED>
+__global__ void __launch_bounds__(kRotaryThreads, sizeof(T) == 2 ? 6 : 4)
+rotary_kernel(const RotaryParams p) {
+  extern __shared__ __align__(16) float2 cs[];  // [block_tokens][half]
+  __shared__ double s_pos[kRotaryTokens];
+  __shared__ long long s_page[kRotaryTokens];  // PAGED: the token's first element of the pools, -1: it has no place
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int t0 = blockIdx.x * p.block_tokens, n = min(p.block_tokens, p.tokens - t0);
+  const int units = n * p.rows * (int)p.per;
+  Piece<T, WIDE> x[kRotaryUnits], y[kRotaryUnits];
+  auto load = [&](int idx0) {
+#pragma unroll
+    for (int b = 0; b < kRotaryUnits; ++b) {
+      const int idx = idx0 + b * kRotaryThreads;
+      if (idx >= units) break;
+      const UnitPlace w = unit_place<WIDE>(p, idx);
+      const long long t = t0 + w.token;
+      const T* src;
+      if (w.head < p.heads) src = static_cast<const T*>(p.q) + t * p.ldq + w.head * p.d;
+      else if (!PAGED || w.head < p.heads + p.kv_heads) src = static_cast<const T*>(p.k) + t * p.ldk + (w.head - p.heads) * p.d;
+      else src = static_cast<const T*>(p.v) + t * p.ldv + (w.head - p.heads - p.kv_heads) * p.d;
+      x[b].load(src + w.first);
+      if (w.second >= 0) y[b].load(src + w.second);
+    }
+  };
+  load(tid);  // on their way while the block works out its positions
+  block_angles<PAGED>(p, t0, n, s_pos, s_page, cs);
   for (int idx0 = tid; idx0 < units;) {
 #pragma unroll
     for (int b = 0; b < kRotaryUnits; ++b) {
@@ -219,6 +225,82 @@ rotary_kernel(const RotaryParams p) {
   }
 }
 
+// The same for prompts of many heads whose units are a power of two (at most a warp): a warp takes a token, and a lane the same unit of every head, so that its cosines
+// and sines stay in registers and a head costs its loads, products and stores, where the places of units in the kernel above take a third of its instructions.
+// 15000 tokens of 32 heads of 64, half of each turned, fp16: 21.5 us, 5.7 TB/s (26.7 there); 7900 tokens, 32 heads of 128 turned and 8 filed with their values: 34.5 us, 5.6 TB/s (42.3).
+// With fewer units of a token, or fewer tokens, a warp has too little on its way: 15000 tokens of 24 heads of 64 (96 units) 27 us and 25 there, 1300 tokens of 40 heads
+// of 128 (320 units) 14 and 12, 5000 of them 29 and 27, 8000 33 and 37 (with the launch). fp32 is bound by memory there already (8000 tokens: 68 and 63).
+template <typename T, bool HALVES, bool PAGED>
+__global__ void __launch_bounds__(kRotaryThreads, 4)
+rotary_heads_kernel(const RotaryParams p) {
+  static_assert(kRotaryThreads / 32 == kRotaryTokens, "a warp a token");
+  constexpr int U = HALVES ? 2 : 4;                     // heads of a lane on their way
+  extern __shared__ __align__(16) float2 cs[];          // [kRotaryTokens][half]
+  __shared__ double s_pos[kRotaryTokens];
+  __shared__ long long s_page[kRotaryTokens];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5, shift = 31 - __clz(p.per), step = 32 >> shift;
+  const int t0 = blockIdx.x * kRotaryTokens, n = min(kRotaryTokens, p.tokens - t0);
+  const long long t = t0 + i;
+  const int u = lane & (int)(p.per - 1), mine = lane >> shift;
+  const bool turned = u * (HALVES ? 8 : 4) < p.half, two = HALVES && turned;
+  const int first = HALVES && !turned ? p.half + u * 8 : u * 8;
+  // kinds of heads: queries, keys, (PAGED) values
+  const T* src = nullptr;
+  T* dst = nullptr;
+  long long out = 0;  // elements between heads
+  int kind = -1, heads = 0, h = 0;
+  Piece<T, true> x[U], y[U];
+  auto more = [&]() {  // heads h and following of a kind; false: none is left
+    while (h >= heads) {
+      if (++kind == (PAGED ? 3 : 2)) return false;
+      heads = kind ? p.kv_heads : p.heads;
+      h = 0;
+      src = (kind == 0 ? static_cast<const T*>(p.q) + t * p.ldq : kind == 1 ? static_cast<const T*>(p.k) + t * p.ldk : static_cast<const T*>(p.v) + t * p.ldv) + first;
+    }
+    return true;
+  };
+  auto load = [&]() {
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      const int head = h + e * step + mine;
+      if (head >= heads) break;
+      x[e].load(src + head * p.d);
+      if (two) y[e].load(src + head * p.d + p.half);
+    }
+  };
+  const bool any = i < n && more();
+  if (any) load();  // on their way while the block works out its positions
+  block_angles<PAGED>(p, t0, n, s_pos, s_page, cs);
+  if (!any) return;
+  constexpr int P = HALVES ? 8 : 4;
+  float4 c[P / 2];
+  if (turned) {
+#pragma unroll
+    for (int e = 0; e < P / 2; ++e) c[e] = *reinterpret_cast<const float4*>(cs + i * p.half + u * P + 2 * e);
+  }
+  const bool placed = !PAGED || s_page[i] >= 0, known = !PAGED || s_pos[i] >= 0;
+  do {
+    if (kind == 0) dst = static_cast<T*>(p.q_out) + t * p.ldq_out + first, out = p.d;
+    else if (!PAGED) dst = static_cast<T*>(p.k_out) + t * p.ldk_out + first, out = p.d;
+    else dst = static_cast<T*>(kind == 1 ? p.keys : p.values) + s_page[i] + first, out = (long long)p.d << p.s.page_shift;
+    if (kind ? placed : known) {
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const int head = h + e * step + mine;
+        if (head >= heads) break;
+        if (turned && (!PAGED || kind < 2)) turn(x[e], y[e], HALVES, reinterpret_cast<const float2*>(c));
+        x[e].store(dst + head * out);
+        if (two) y[e].store(dst + head * out + p.half);
+      }
+    }
+    h += U * step;
+    if (!more()) break;
+    load();
+  } while (true);
+}
+
 template <typename T, bool PAGED>
 int launch_rotary(ttb_ctx* ctx, RotaryParams& p, const char* what) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
@@ -231,8 +313,17 @@ int launch_rotary(ttb_ctx* ctx, RotaryParams& p, const char* what) {
   p.block_tokens = std::max(1, std::min(std::min(kRotaryTokens, 2 * kRotaryUnits * kRotaryThreads / std::max(1, units)), p.tokens / (4 * ctx->sm_count)));
   p.per_magic = (unsigned)(((1ull << 32) + p.per - 1) / p.per);
   p.rows_magic = p.block_tokens == 1 ? 0 : (unsigned)(((1ull << 32) + p.rows - 1) / p.rows);
+  const bool by_heads = sizeof(T) == 2 && wide && p.per <= 32 && (p.per & (p.per - 1)) == 0 && (int64_t)p.rows * p.per >= 256 && p.tokens >= 48 * ctx->sm_count;
+  if (by_heads) p.block_tokens = kRotaryTokens;
   const dim3 grid((unsigned)((p.tokens + p.block_tokens - 1) / p.block_tokens));
   const size_t smem = (size_t)p.block_tokens * p.half * sizeof(float2);
+  if constexpr (sizeof(T) == 2) {
+    if (by_heads) {
+      if (p.interleaved) launch_pdl(rotary_heads_kernel<T, false, PAGED>, grid, dim3(kRotaryThreads), smem, ctx->stream, p);
+      else launch_pdl(rotary_heads_kernel<T, true, PAGED>, grid, dim3(kRotaryThreads), smem, ctx->stream, p);
+      return launched(ctx, what);
+    }
+  }
   if (wide) launch_pdl(rotary_kernel<T, true, PAGED>, grid, dim3(kRotaryThreads), smem, ctx->stream, p);
   else launch_pdl(rotary_kernel<T, false, PAGED>, grid, dim3(kRotaryThreads), smem, ctx->stream, p);
   return launched(ctx, what);
