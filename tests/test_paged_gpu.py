@@ -327,6 +327,34 @@ def test_attention_with_scores_far_apart(new):
     assert ((got.double() - want).abs() <= off + 2.0 ** -8 * want.abs().amax()).all()
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("page,past,new,heads,kv,d,causal", [
+    (64, [0], [314], 12, 3, 64, True), (16, [616], [336], 33, 1, 128, False), (128, [0, 1054], [667, 20], 8, 2, 128, False), (16, [0, 4000], [1, 300], 40, 1, 64, True),
+    (16, [300, 2000, 77], [1, 1, 1], 24, 1, 128, True)])
+def test_attention_with_few_keys_that_count(page, past, new, heads, kv, d, causal, dt):
+    """Scores spread by some 60: the reference is raised time and again, with no more than one rounding of a probability."""
+    dtype, scale = DT[dt], 0.3
+    pool = Pool(sum(new) + d, dtype, past, new, kv, d, page)
+    pool.fill_new(dtype, kv, d)
+    q = randn(pool.g, sum(new), heads, d, dtype=dtype) * 4
+    got = tt.paged_attention(q, *pool.args(), causal=causal, scale=scale)
+    assert status() == _capi.OK
+    want, off = attended(q, pool, causal, scale)
+    # A score is off by d / 16 + 1 roundings (of a step at most: the products are summed 16 at a time) of a sum that the moduli bound, and two roundings of the scaled one: a
+    # probability by that much of itself, and their sum as well.
+    t = 0
+    for b, (p, n) in enumerate(zip(past, new)):
+        k, v = (x.double().repeat_interleave(heads // kv, 1) for x in pool.held(b, p + n))
+        most = torch.einsum("ihd,jhd->hij", q[t:t + n].double().abs(), k.abs()).amax() * scale
+        score = torch.einsum("ihd,jhd->hij", q[t:t + n].double(), k) * scale
+        if causal:
+            score.masked_fill_(torch.arange(p + n, device=DEV) > p + torch.arange(n, device=DEV)[:, None], -float("inf"))
+        off[t:t + n] += 2 * (d // 16 + 3) * 2.0 ** -23 * most * torch.einsum("hij,jhd->ihd", score.softmax(-1), v.abs())
+        t += n
+    far = (got.double() - want).abs()
+    assert (far <= off).all(), f"{(far / off).max().item():.3g} times the tolerance"
+
+
 def test_attention_of_nothing_and_of_padded_calls():
     pool = Pool(5, torch.float16, [10, 0, 4], [0, 0, 0], 2, 64, 16)
     q = torch.full((4, 2, 64), float("nan"), dtype=torch.float16, device=DEV)
