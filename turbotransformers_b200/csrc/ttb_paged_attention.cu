@@ -572,7 +572,7 @@ template <typename T, int D>
 int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, Params& p) {
   // Which kernels, and the rows of a tile of the one for few. The host knows the sum of the new tokens only. With no more tokens than sequences, tiles of a token's rows (up to 32)
   // take all of them, a sequence of several tokens several tiles. Otherwise tiles of an average sequence's rows, 16 at most, and the sequences that have more go
-  // to the kernel for many (16 requests of 3 to 6 tokens, 8 heads to a key head, over up to 16000: 153 us there, 171 with those of 32 rows in this one).
+  // to the kernel for many (16 requests of 3 to 6 tokens, 8 heads to a key head, over up to 16000: 144 to 151 us there, 171 with those of 32 rows in this one).
   const int64_t tokens = p.s.tokens, B = kv->B, each = (tokens + B - 1) / B * p.group;
   const int64_t need = std::max<int64_t>(p.group, std::min<int64_t>(each, 16));
   const int groups = need <= 8 ? 1 : need <= 16 ? 2 : 4, few = 8 * groups / p.group;

@@ -13,9 +13,9 @@
 //                 are whole numbers (of log2), so that probabilities that are brought to a new one are not rounded a second time.
 // A tile's output is written while the next one's first scores are made. Every wait is bounded. The probabilities are rounded to the values' 16 bits, as in the kernel for few
 // rows; their sums are not.
-// 4000 tokens over 12000, 32 heads of 128 on 8 key heads, bf16: 900 us, 1.02 PFLOP/s of products that the mask leaves; a pair of units takes 4400 cycles, of which the products
+// 4000 tokens over 12000, 32 heads of 128 on 8 key heads, bf16: 890 us, 1.03 PFLOP/s of products that the mask leaves; a pair of units takes 4400 cycles, of which the products
 // are 2050 and a set's exponentials alone 1024 on their own unit, with the conversions, sums and tensor memory traffic of 256 rows beside them. 16 requests of 3 to 6
-// tokens over up to 16000, 64 heads of 128 on 8: 153 us, 4.1 TB/s: two tiles of values are the most that fit beside the queries, and their way from memory shows
+// tokens over up to 16000, 64 heads of 128 on 8: 144 to 151 us, 4.2 to 4.4 TB/s: two tiles of values are the most that fit beside the queries, and their way from memory shows
 // (a third place for keys changed nothing).
 #include <algorithm>
 #include <type_traits>
