@@ -275,6 +275,7 @@ STEPS = [
     (16, [255, 10], [1, 1], 32, 1, 64, False), (16, [300, 0, 77], [1, 1, 1], 33, 1, 64, True), (16, [90, 5, 300, 0, 0, 2], [0, 6, 0, 0, 0, 0], 24, 2, 64, True),
     (32, [90, 5, 300, 40], [1, 0, 3, 0], 40, 2, 128, True), (16, [10] * 40, [0] * 39 + [40], 4, 4, 64, True), (16, [7000], [7], 16, 1, 64, True), (16, [7000], [8], 32, 2, 64, False),
     (256, [4000], [2], 32, 2, 128, True), (16, [1000], [4], 4, 2, 128, True), (128, [999], [9], 4, 4, 64, True),
+    (16, [1000, 3000], [3, 2], 7, 1, 128, True), (32, [700, 10, 0, 5000], [8, 6, 7, 7], 4, 1, 64, True), (16, [2000, 127, 129], [6, 1, 2], 16, 2, 128, False),
 ]
 
 
