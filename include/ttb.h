@@ -464,9 +464,11 @@ typedef struct ttb_paged_pool {
   void* base;
   int64_t planes, plane_stride, pages, page_stride, page_bytes;
 } ttb_paged_pool;
-/* Room for new_tokens[b] more tokens (0: the row is left alone) of every row, before ttb_paged_append: the lowest free pages, in the rows' order. A row whose
+/* Room for new_tokens[b] more tokens (0: the row is left alone) of every row, before ttb_paged_append: the lowest free pages, in the rows' order. Pages that a row lists
+ * already behind its tokens (it had room for more than it kept, or gave tokens back) are used before others are taken; they are the row's until it is freed. A row whose
  * last page is begun and listed by other rows too gets a page of its own in its place: copies[i] = (from, to), i < B, in the rows' order, (-1, -1) behind the
- * last, for ttb_paged_copy, which goes before the next append. (Of rows that are all of a page's holders the last keeps it.) granted[b] = 1, or 0 where the
+ * last, for ttb_paged_copy, which goes before the next append; pages behind its tokens that other rows list too are replaced without a copy. (Of rows that write and are all of
+ * a page's holders the last keeps it.) granted[b] = 1, or 0 where the
  * pages do not suffice: from the first such row on nothing is granted, so that no later row overtakes it; or where the row of the table is too short. lens is left
  * to the caller, who adds the new tokens when all layers have filed them. */
 int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies);

@@ -1,0 +1,141 @@
+"""The books of a pool of cache pages, over runs in which rows keep fewer tokens than they reserved, give tokens back, are refused and ask again: reference counts say how many
+rows list a page at all times, and nothing is lost."""
+import random
+
+import pytest
+import torch
+
+import turbotransformers_b200 as tt
+from turbotransformers_b200 import _capi
+from turbotransformers_b200._cxx import cxx
+
+pytestmark = pytest.mark.gpu
+torch.set_grad_enabled(False)
+DEV = torch.device("cuda:0")
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def status():
+    return cxx.device_status(0)
+
+
+class Ledger:
+    """Page tables kept by the rules of include/ttb.h, one row and one column after the other."""
+
+    def __init__(self, B, width, pages, page):
+        self.B, self.width, self.pages, self.page = B, width, pages, page
+        self.lens, self.table, self.refs = [0] * B, [[-1] * width for _ in range(B)], [0] * pages
+
+    def counted(self):
+        refs = [0] * self.pages
+        for p in (p for row in self.table for p in row if p >= 0):
+            refs[p] += 1
+        return refs
+
+    def fork(self, parents):
+        self.table = [list(self.table[p]) if p >= 0 else [-1] * self.width for p in parents]
+        self.lens = [self.lens[p] if p >= 0 else 0 for p in parents]
+        self.refs = self.counted()
+
+    def reserve(self, new):
+        before, free = list(self.refs), [p for p, r in enumerate(self.refs) if r == 0]
+        granted, copies, stopped = [], [], False
+        for b, n in enumerate(new):
+            if n == 0:
+                granted.append(1)
+                continue
+            have, want = -(-self.lens[b] // self.page), -(-(self.lens[b] + n) // self.page)
+            if want > self.width:
+                granted.append(0)
+                continue
+            begun = self.lens[b] % self.page != 0
+            listed = lambda p: 0 <= p < self.pages and before[p] > 0  # noqa: E731
+            takes = [c for c in range(have - begun, want) if not listed(self.table[b][c]) or self.refs[self.table[b][c]] > 1]
+            stopped |= len(takes) > len(free)
+            granted.append(0 if stopped else 1)
+            if stopped:
+                continue
+            for c in takes:
+                old, fresh = self.table[b][c], free.pop(0)
+                if begun and c == have - 1:
+                    copies.append([old, fresh])
+                if listed(old):
+                    self.refs[old] -= 1
+                self.table[b][c] = fresh
+                self.refs[fresh] = 1
+        assert self.refs == self.counted()
+        return granted, copies + [[-1, -1]] * (self.B - len(copies))
+
+    def compact(self):
+        used = sum(r > 0 for r in self.refs)
+        to = dict(zip([p for p in range(used, self.pages) if self.refs[p] > 0], [p for p in range(used) if self.refs[p] == 0]))
+        self.table = [[to.get(p, p) for p in row] for row in self.table]
+        self.refs = self.counted()
+        return used
+
+
+def same(ledger, tensors):
+    table, lens, refs = (x.tolist() for x in tensors)
+    assert table == ledger.table and lens == ledger.lens and refs == ledger.refs
+
+
+def test_rows_that_keep_fewer_tokens_than_they_reserved_lose_no_page():
+    """15 tokens cached, 5 proposed three times and none kept, then the row is freed."""
+    t = ints([[-1] * 4]), ints([0]), ints([0] * 6)
+    tt.paged_reserve(*t, ints([15]), 16)
+    t[1].fill_(15)
+    for _ in range(3):
+        granted, copies = tt.paged_reserve(*t, ints([5]), 16)
+        assert granted.tolist() == [1] and copies.tolist() == [[-1, -1]]
+        assert t[0].tolist() == [[0, 1, -1, -1]] and t[2].tolist() == [1, 1, 0, 0, 0, 0]
+    tt.paged_fork(*t, ints([-1]))
+    assert t[2].tolist() == [0] * 6 and status() == _capi.OK
+
+
+def test_pages_reserved_and_then_shared_are_each_rows_own_when_written():
+    """A row with pages in hand is forked: of the two that go on, the first gets its own in their place, the last keeps them."""
+    ledger = Ledger(3, 5, 12, 16)
+    t = ints(ledger.table), ints(ledger.lens), ints(ledger.refs)
+    for new, keep, parents in (([40, 0, 0], [20, 0, 0], [0, 0, 0]), ([30, 30, 0], [1, 13, 0], [0, 1, 2]), ([0, 4, 60], [0, 0, 60], [-1, -1, -1])):
+        granted, copies = tt.paged_reserve(*t, ints(new), 16)
+        want, pairs = ledger.reserve(new)
+        assert granted.tolist() == want == [1, 1, 1] and copies.tolist() == pairs
+        same(ledger, t)
+        t[1].add_(ints(keep))
+        ledger.lens = [a + b for a, b in zip(ledger.lens, keep)]
+        tt.paged_fork(*t, ints(parents))
+        ledger.fork(parents)
+        same(ledger, t)
+    assert t[2].tolist() == [0] * 12 and status() == _capi.OK
+
+
+@pytest.mark.parametrize("B,width,pages,page", [(1, 3, 4, 16), (3, 6, 14, 16), (9, 12, 70, 32), (40, 150, 900, 64), (200, 9, 5000, 256), (1024, 4, 1500, 16)])
+def test_reserve_after_fewer_were_kept_and_after_tokens_were_given_back(B, width, pages, page):
+    rng = random.Random(B * width + pages)
+    ledger = Ledger(B, width, pages, page)
+    t = ints(ledger.table).view(B, width), ints(ledger.lens), ints(ledger.refs)
+    most = width * page
+    for step in range(16):
+        new = [rng.choice([0, 1, 5, rng.randint(1, 2 * page), rng.randint(1, most)]) for _ in range(B)]
+        granted, copies = tt.paged_reserve(*t, ints(new), page)
+        want, pairs = ledger.reserve(new)
+        assert granted.tolist() == want and copies.tolist() == pairs
+        same(ledger, t)
+        keep = [g * rng.choice([n, n, rng.randint(0, n), 0]) for n, g in zip(new, want)]
+        lens = [x + k for x, k in zip(ledger.lens, keep)]
+        ledger.lens = [rng.choice([x, x, x, rng.randint(0, x)]) for x in lens]  # some tokens are given back
+        t[1].copy_(ints(ledger.lens))
+        if step % 3 == 1:
+            parents = [rng.choice([-1, b, b, b, rng.randrange(B)]) for b in range(B)]
+            tt.paged_fork(*t, ints(parents))
+            ledger.fork(parents)
+            same(ledger, t)
+        if step % 5 == 4:
+            used = ledger.compact()
+            assert tt.paged_compact(t[0], t[2], torch.zeros(1, pages, 4, device=DEV)).tolist() == [used]
+            same(ledger, t)
+    tt.paged_fork(*t, ints([-1] * B))
+    assert (t[2] == 0).all() and (t[0] == -1).all() and status() == _capi.OK

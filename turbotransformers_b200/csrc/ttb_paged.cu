@@ -372,51 +372,108 @@ struct Tables {
   int* status;
 };
 
-// Pages for new[b] more tokens of every row (see ttb.h for the rules). One block; thread b decides for row b, then a warp a row fills the table in.
+// Pages for new[b] more tokens of every row (see ttb.h for the rules). One block; thread b decides for row b.
+// A row writes to the columns from the page that it has begun, or else the next one, to the last that its new tokens reach. What it lists there (it may have kept fewer tokens
+// than it once had room for) stays its own; a page in any of them is left for a fresh one only where other rows list it too, unless the row is the last of holders that all
+// write. A row's thread looks at its first columns, warps at what is beyond them (a prompt's): those go by keeper[page], made before the first count changes.
+// 64 rows over 1300 pages, most of them sharing the page that they go on in: 8 us with cold caches.
 // free_list [pages], sharers [pages], keeper [pages]: scratch, not initialised.
+constexpr int kOwnColumns = 2;
+constexpr int kNobody = -1, kUncounted = -2, kWhoever = INT_MAX;  // keeper: all holders leave it; its count is zero, so that it is free; one row alone lists it
 __global__ void __launch_bounds__(kManageThreads, 1)
 paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page_tokens, int32_t* granted, int32_t* copies, int* free_list, int* sharers,
                      int* keeper) {
   __shared__ int scratch[33];
-  __shared__ int s_first[kMaxSequences], s_want[kMaxSequences], s_base[kMaxSequences];
+  __shared__ int s_first[kMaxSequences], s_want[kMaxSequences], s_at[kMaxSequences];
   pdl_trigger();
   pdl_wait();
-  const int b = threadIdx.x;
-  int len = 0, add = 0, have = 0, want = 0, last = -1, last_refs = 0;
-  bool fits = false, open = false;
+  const int b = threadIdx.x, lane = threadIdx.x & 31;
+  auto listed = [&](int row, int col) {  // -1: nothing that is in the pool
+    const int page = t.table[row * t.stride + col];
+    return page >= 0 && page < t.pages ? page : -1;
+  };
+  int len = 0, add = 0, first = 0, want = 0;
+  bool fits = false, begun = false;
   if (b < t.B) {
     len = t.lens[b];
     add = fresh[b];
     const long long cap = (long long)t.width * page_tokens;
     fits = len >= 0 && add >= 0 && (long long)len + add <= cap;
     if (len < 0 || add < 0 || len > cap) bad_index(t.status);
-    if (fits) {
-      have = (len + page_tokens - 1) / page_tokens;
+    if (fits && add > 0) {
+      begun = len % page_tokens != 0;
+      first = len / page_tokens;
       want = (len + add + page_tokens - 1) / page_tokens;
-      if (add > 0 && len % page_tokens != 0) {
-        last = t.table[b * t.stride + have - 1];
-        open = last >= 0 && last < t.pages;
-        if (!open) bad_index(t.status);
-      }
     }
-    if (open) {
-      last_refs = t.refs[last];
-      sharers[last] = 0;
-      keeper[last] = -1;
-    }
+    s_first[b] = first;
+    s_want[b] = want;
+    s_at[b] = 0;
   }
+  int page[kOwnColumns], refs[kOwnColumns];
+#pragma unroll
+  for (int i = 0; i < kOwnColumns; ++i) page[i] = first + i < want ? listed(b, first + i) : -1;
+#pragma unroll
+  for (int i = 0; i < kOwnColumns; ++i) refs[i] = page[i] >= 0 ? t.refs[page[i]] : 0;
+  if (begun && page[0] < 0) bad_index(t.status);
+  auto begin = [&](int page, int refs) {
+    if (page < 0) return;
+    sharers[page] = 0;
+    keeper[page] = refs > 1 ? kNobody : refs == 1 ? kWhoever : kUncounted;
+  };
+#pragma unroll
+  for (int i = 0; i < kOwnColumns; ++i) begin(page[i], refs[i]);
+  __threadfence_block();
+  const bool far = __syncthreads_or(want - first > kOwnColumns);
+  auto beyond = [&](auto&& f) {  // what is beyond the rows' first columns
+    for (int row = threadIdx.x >> 5; row < t.B; row += kManageThreads / 32)
+      for (int col = s_first[row] + kOwnColumns + lane; col < s_want[row]; col += 32) f(row, listed(row, col));
+  };
+  if (far) {
+    beyond([&](int, int page) { begin(page, page >= 0 ? t.refs[page] : 0); });
+    __threadfence_block();
+    __syncthreads();
+  }
+  auto share = [&](int row, int page, int refs) {
+    if (page < 0 || refs <= 1) return;
+    atomicAdd(sharers + page, 1);
+    atomicMax(keeper + page, row);
+  };
+#pragma unroll
+  for (int i = 0; i < kOwnColumns; ++i) share(b, page[i], refs[i]);
+  if (far) beyond([&](int row, int page) { share(row, page, page >= 0 ? t.refs[page] : 0); });
   __threadfence_block();
   __syncthreads();
-  if (open) {
-    atomicAdd(sharers + last, 1);
-    atomicMax(keeper + last, b);
+  // Which columns take a page. (A page that is begun holds the row's tokens, whatever its count says.)
+  bool takes[kOwnColumns];
+  int own = 0, need;
+#pragma unroll
+  for (int i = 0; i < kOwnColumns; ++i) {
+    const bool holds = begun && i == 0;
+    if (refs[i] > 1) takes[i] = !(__ldcg(sharers + page[i]) == refs[i] && __ldcg(keeper + page[i]) == b);
+    else takes[i] = first + i < want && refs[i] != 1 && !holds;
+    own += takes[i];
   }
-  __threadfence_block();
-  __syncthreads();
-  // rows that are all of a page's holders: the last of them keeps it
-  bool copy = open && last_refs > 1 && !(__ldcg(sharers + last) == last_refs && __ldcg(keeper + last) == b);
+  need = own;
+  auto passed = [&](int row, int page) {  // of a column beyond, when the keepers are settled
+    if (page < 0) return true;
+    const int k = __ldcg(keeper + page);
+    return k != kWhoever && k != row;
+  };
+  if (far) {
+    beyond([&](int, int page) {
+      if (page < 0) return;
+      const int refs = t.refs[page];
+      if (refs > 1 && __ldcg(sharers + page) != refs) keeper[page] = kNobody;
+    });
+    __threadfence_block();
+    __syncthreads();
+    beyond([&](int row, int page) {
+      if (passed(row, page)) atomicAdd(s_at + row, 1);
+    });
+    __syncthreads();
+    if (b < t.B) need += s_at[b];
+  }
   const bool writes = add > 0;
-  const int need = writes && fits ? want - have + (copy ? 1 : 0) : 0;
   int total, found = 0;
   const int before = block_scan(need, scratch, &total);
   // the lowest free pages, as many as are needed
@@ -434,27 +491,42 @@ paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page
   __threadfence_block();
   __syncthreads();
   const bool ok = !writes || (fits && (long long)before + need <= found);
-  copy = copy && ok;
+  const bool copy = ok && begun && takes[0];
   int n_copies;
   const int c = block_scan(copy ? 1 : 0, scratch, &n_copies);
   if (b < t.B) {
     granted[b] = ok;
-    s_first[b] = copy ? have - 1 : have;
-    s_want[b] = ok && writes ? want : 0;
-    s_base[b] = before;
+    if (!ok) s_want[b] = first;  // nothing to fill in
+    s_at[b] = before + own;
     if (copy) {
-      copies[2 * c] = last;
+      copies[2 * c] = page[0];
       copies[2 * c + 1] = free_list[before];
-      atomicSub(t.refs + last, 1);
     }
     if (b >= n_copies) copies[2 * b] = copies[2 * b + 1] = -1;
+    int at = before;
+#pragma unroll
+    for (int i = 0; i < kOwnColumns; ++i)
+      if (ok && takes[i]) {
+        const int taken = free_list[at++];
+        t.table[b * t.stride + first + i] = taken;
+        t.refs[taken] = 1;
+        if (refs[i] > 0) atomicSub(t.refs + page[i], 1);
+      }
   }
+  if (!far) return;
   __syncthreads();
   for (int row = threadIdx.x >> 5; row < t.B; row += kManageThreads / 32)
-    for (int col = s_first[row] + (threadIdx.x & 31); col < s_want[row]; col += 32) {
-      const int page = free_list[s_base[row] + col - s_first[row]];
-      t.table[row * t.stride + col] = page;
-      t.refs[page] = 1;
+    for (int c0 = s_first[row] + kOwnColumns, at = s_at[row]; c0 < s_want[row]; c0 += 32) {
+      const int col = c0 + lane, had = col < s_want[row] ? listed(row, col) : -1;
+      const bool take = col < s_want[row] && passed(row, had);
+      const unsigned mask = __ballot_sync(0xffffffffu, take);
+      if (take) {
+        const int taken = free_list[at + __popc(mask & ((1u << lane) - 1))];
+        t.table[row * t.stride + col] = taken;
+        t.refs[taken] = 1;
+        if (had >= 0 && __ldcg(keeper + had) != kUncounted) atomicSub(t.refs + had, 1);
+      }
+      at += __popc(mask);
     }
 }
 
