@@ -469,7 +469,8 @@ typedef struct ttb_paged_pool {
  * last page is begun and listed by other rows too gets a page of its own in its place: copies[i] = (from, to), i < B, in the rows' order, (-1, -1) behind the
  * last, for ttb_paged_copy, which goes before the next append; pages behind its tokens that other rows list too are replaced without a copy. (Of rows that write and are all of
  * a page's holders the last keeps it.) granted[b] = 1, or 0 where the
- * pages do not suffice: from the first such row on nothing is granted, so that no later row overtakes it; or where the row of the table is too short. lens is left
+ * pages do not suffice: from the first such row on nothing is granted, so that no later row overtakes it; or where the row of the table is too short, or the row is not one
+ * (a length that the table cannot hold or a negative number of new tokens, which are TTB_ERR_BAD_INDEX, as is a row without a page for its last token). lens is left
  * to the caller, who adds the new tokens when all layers have filed them. */
 int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies);
 /* Row b becomes what row parents[b] was (its pages are shared, not copied), for beams that follow their parents and requests that fork; -1 frees the row: its

@@ -139,3 +139,18 @@ def test_reserve_after_fewer_were_kept_and_after_tokens_were_given_back(B, width
             same(ledger, t)
     tt.paged_fork(*t, ints([-1] * B))
     assert (t[2] == 0).all() and (t[0] == -1).all() and status() == _capi.OK
+
+
+def test_bad_rows_are_not_granted_and_left_alone():
+    """Row by row: its last page outside the pool, -1 (begun, and full), a negative number of tokens, a negative length, lengths beyond the table; the good rows among them get theirs."""
+    table = [[3, 9], [-1, -1], [-1, -1], [1, -1], [-1, -1], [2, 4], [2, 4], [-1, -1], [1, -1]]
+    lens, new, refs = [20, 5, 16, 10, -4, 33, 2 ** 31 - 1, 0, 10], [1, 1, 1, -3, 0, 0, 1, 3, 8], [0, 2, 2, 1, 2, 0]
+    t = ints(table), ints(lens), ints(refs)
+    granted, copies = tt.paged_reserve(*t, ints(new), 16)
+    assert status() == _capi.ERR_BAD_INDEX
+    assert granted.tolist() == [0, 0, 0, 0, 0, 0, 0, 1, 0]  # (the last row wants two pages, of which row 7 has left one: it is not bad)
+    assert copies.tolist() == [[-1, -1]] * 9
+    assert t[0].tolist() == table[:7] + [[0, -1]] + table[8:] and t[1].tolist() == lens and t[2].tolist() == [1, 2, 2, 1, 2, 0]
+    for bad in ([-3], [-2 ** 31]):  # so that lens += new * granted never takes tokens away
+        t = ints([[0, -1]]), ints([10]), ints([1, 0])
+        assert tt.paged_reserve(*t, ints(bad), 16)[0].tolist() == [0] and status() == _capi.ERR_BAD_INDEX

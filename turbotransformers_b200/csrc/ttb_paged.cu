@@ -393,18 +393,20 @@ paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page
     return page >= 0 && page < t.pages ? page : -1;
   };
   int len = 0, add = 0, first = 0, want = 0;
-  bool fits = false, begun = false;
+  bool fits = false, begun = false, bad = false;  // bad: the row's length or what is asked for is no number of tokens, or its last page is none
   if (b < t.B) {
     len = t.lens[b];
     add = fresh[b];
     const long long cap = (long long)t.width * page_tokens;
     fits = len >= 0 && add >= 0 && (long long)len + add <= cap;
-    if (len < 0 || add < 0 || len > cap) bad_index(t.status);
+    bad = len < 0 || add < 0 || len > cap;
     if (fits && add > 0) {
       begun = len % page_tokens != 0;
       first = len / page_tokens;
-      want = (len + add + page_tokens - 1) / page_tokens;
+      bad = len > 0 && listed(b, first - (begun ? 0 : 1)) < 0;
+      if (!bad) want = (len + add + page_tokens - 1) / page_tokens;
     }
+    if (bad) bad_index(t.status);
     s_first[b] = first;
     s_want[b] = want;
     s_at[b] = 0;
@@ -414,7 +416,6 @@ paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page
   for (int i = 0; i < kOwnColumns; ++i) page[i] = first + i < want ? listed(b, first + i) : -1;
 #pragma unroll
   for (int i = 0; i < kOwnColumns; ++i) refs[i] = page[i] >= 0 ? t.refs[page[i]] : 0;
-  if (begun && page[0] < 0) bad_index(t.status);
   auto begin = [&](int page, int refs) {
     if (page < 0) return;
     sharers[page] = 0;
@@ -490,7 +491,7 @@ paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page
   }
   __threadfence_block();
   __syncthreads();
-  const bool ok = !writes || (fits && (long long)before + need <= found);
+  const bool ok = !bad && (!writes || (fits && (long long)before + need <= found));
   const bool copy = ok && begun && takes[0];
   int n_copies;
   const int c = block_scan(copy ? 1 : 0, scratch, &n_copies);

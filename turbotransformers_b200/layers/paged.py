@@ -211,7 +211,7 @@ def _pool(pool):
 def paged_reserve(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, new_tokens: torch.Tensor, page_tokens: int):
     """Room for new_tokens[b] more tokens of every row of the page table: pages that the row lists already behind its tokens, then the lowest free ones (those of refs 0),
     which are taken into the table. A row that would write to a page that other rows list too gets one of its own in its place. Returns (granted int32 [sequences], copies int32 [sequences, 2]); hand the copies to paged_copy before the new
-    tokens are filed. A row that is not granted (0) has been left alone: the pool is full, or its row of the table."""
+    tokens are filed. A row that is not granted (0) has been left alone: the pool is full, or its row of the table, or the row or its number of tokens is bad (see device_status)."""
     device, t = _tables(table, lens, refs)
     new = _index(new_tokens, "new_tokens", t[2], device)
     granted, copies = torch.empty_like(new_tokens), new_tokens.new_empty((t[2], 2))
