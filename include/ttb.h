@@ -452,7 +452,7 @@ int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const v
                         void* out, int64_t ldo);
 
 /* The pages of B sequences: table int32 [B, width] (stride between rows), -1 behind a row's last page; lens int32 [B], the tokens cached; refs int32 [pages], how
- * many rows list a page (0: it is free). */
+ * many rows list a page (0: it is free). B * width < 2^31. */
 typedef struct ttb_paged_tables {
   int32_t* table;
   int64_t stride, B, width;

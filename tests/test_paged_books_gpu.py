@@ -154,3 +154,16 @@ def test_bad_rows_are_not_granted_and_left_alone():
     for bad in ([-3], [-2 ** 31]):  # so that lens += new * granted never takes tokens away
         t = ints([[0, -1]]), ints([10]), ints([1, 0])
         assert tt.paged_reserve(*t, ints(bad), 16)[0].tolist() == [0] and status() == _capi.ERR_BAD_INDEX
+
+
+def test_a_table_whose_pages_could_not_be_counted_is_refused(ctx):
+    """Rows that want 2^31 pages together: refused before anything is launched (the table that is handed over here has two entries)."""
+    table, lens, refs, new, granted = ints([[-1, -1]]), ints([0] * 1024), ints([0]), ints([0] * 1024), ints([0] * 1024)
+    copies = ints([[0, 0]] * 1024)
+    launches = _capi.lib().ttb_launch_count(ctx.h)
+    for B, width, page in ((1024, 1 << 21, 16), (3, (1 << 30) - 1, 1), (33, 1 << 26, 16)):
+        assert B * width >= 1 << 31
+        tables = dict(table=table, stride=width, B=B, width=width, lens=lens, refs=refs, pages=1)
+        with pytest.raises(_capi.TTBError):
+            ctx.paged_reserve(tables, new, page, granted, copies)
+    assert _capi.lib().ttb_launch_count(ctx.h) == launches

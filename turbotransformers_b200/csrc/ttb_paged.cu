@@ -753,6 +753,8 @@ extern "C" int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* a, const 
   const int bad = check_tables(ctx, "paged_reserve", a, &t);
   if (bad) return bad;
   TTB_REQUIRE(ctx, page_tokens > 0 && page_tokens <= (1ll << 20) && page_tokens * a->width <= (1ll << 30), "paged_reserve: bad page size");
+  // the pages that all rows want together are summed in 32 bits
+  TTB_REQUIRE(ctx, a->B * a->width < (1ll << 31), "paged_reserve: a table has fewer than 2^31 entries");
   if (a->B == 0) return TTB_OK;
   TTB_REQUIRE(ctx, a->lens && new_tokens && granted && copies, "paged_reserve: null pointer");
   DeviceGuard g(ctx->device);
