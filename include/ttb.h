@@ -420,7 +420,9 @@ int ttb_rotary(ttb_ctx* ctx, const ttb_rotary_args* args);
  *                  256; d 64 or 128
  *   table        : int32 [B, table_width], table_stride between rows: token j of sequence b is in page table[b][j / page_tokens], row j % page_tokens
  *   cu_seqlens   : int32 [B+1]: sequence b's new tokens are rows [cu[b], cu[b+1]) of the call's q, k, v; rows outside [cu[0], cu[B]) are left alone
- *   past_lens    : int32 [B]: tokens of sequence b that were cached before: new token i is token past + i */
+ *   past_lens    : int32 [B]: tokens of sequence b that were cached before: new token i is token past + i
+ *   room         : int32 [B] or NULL: sequences with 0 are passed over, as if they had no new tokens: nothing is filed, and their rows of the outputs are left alone
+ *                  (ttb_paged_reserve's granted, so that a row without pages does no harm and the others go on) */
 typedef struct ttb_paged_kv {
   void *keys, *values;
   int64_t page_stride, pages, kv_heads, page_tokens, d;
@@ -428,6 +430,7 @@ typedef struct ttb_paged_kv {
   int64_t table_stride, table_width;
   const int32_t *cu_seqlens, *past_lens;
   int64_t B;
+  const int32_t* room;
 } ttb_paged_kv;
 /* The rotary positions of ttb_paged_append: k is turned by its tokens' places in their sequences, and so is q[tokens, heads, d] into q_out (heads = 0: none). */
 typedef struct ttb_paged_rotary {
@@ -452,12 +455,14 @@ int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const v
                         void* out, int64_t ldo);
 
 /* The pages of B sequences: table int32 [B, width] (stride between rows), -1 behind a row's last page; lens int32 [B], the tokens cached; refs int32 [pages], how
- * many rows list a page (0: it is free). B * width < 2^31. */
+ * many rows list a page (0: it is free). B * width < 2^31. room int32 [B] or NULL: receives
+ * what ttb_paged_reserve grants as well, a place that stays while `granted` may be another's every step. */
 typedef struct ttb_paged_tables {
   int32_t* table;
   int64_t stride, B, width;
   int32_t *lens, *refs;
   int64_t pages;
+  int32_t* room;
 } ttb_paged_tables;
 /* A stack's pages: `planes` (of each layer the keys and the values) of `pages` pages of page_bytes; strides in bytes; everything a multiple of 16. */
 typedef struct ttb_paged_pool {
@@ -471,7 +476,7 @@ typedef struct ttb_paged_pool {
  * a page's holders the last keeps it.) granted[b] = 1, or 0 where the
  * pages do not suffice: from the first such row on nothing is granted, so that no later row overtakes it; or where the row of the table is too short, or the row is not one
  * (a length that the table cannot hold or a negative number of new tokens, which are TTB_ERR_BAD_INDEX, as is a row without a page for its last token). lens is left
- * to the caller, who adds the new tokens when all layers have filed them. */
+ * to the caller, who adds the new tokens that were granted when all layers have filed them. */
 int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies);
 /* Row b becomes what row parents[b] was (its pages are shared, not copied), for beams that follow their parents and requests that fork; -1 frees the row: its
  * length becomes 0. Any number of rows may have the same parent. A parent outside [-1, B) leaves its row as it is. */

@@ -167,3 +167,124 @@ def test_a_table_whose_pages_could_not_be_counted_is_refused(ctx):
         with pytest.raises(_capi.TTBError):
             ctx.paged_reserve(tables, new, page, granted, copies)
     assert _capi.lib().ttb_launch_count(ctx.h) == launches
+
+
+# ---------------------------------------------------------------------------------------------------
+# rows that were not granted
+# ---------------------------------------------------------------------------------------------------
+def rows(g, n, heads, d, dtype):
+    return torch.randn(n, heads, d, generator=g, device=DEV, dtype=dtype)
+
+
+def cumulative(new):
+    return ints([sum(new[:i]) for i in range(len(new) + 1)])
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 0, 1], [3, 2, 1], [200, 7, 130], [4, 300, 0]])
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_sequences_without_room_are_passed_over(new, d, dtype):
+    """Nothing of them is filed, their rows of the outputs are as they were, the others get what they get without them; and no page or length of theirs is reported."""
+    heads, kv, page, past = 4, 2, 16, [33, 20, 70]
+    g = torch.Generator(DEV).manual_seed(sum(new) + d)
+    table = ints([[b * 20 + c for c in range(20)] for b in range(3)])
+    table[1] = 2 ** 30  # the row without room has no pages, and more tokens than the table lists
+    lens, cu = ints(past), cumulative(new)
+    lens[1] = 20 * page - 1
+    pool = torch.randn(2, 60, kv, page, d, generator=g, device=DEV, dtype=dtype)
+    room, freqs = ints([1, 0, 7]), 10.0 ** -torch.arange(d // 2, dtype=torch.float64, device=DEV)
+    q, k, v = (rows(g, sum(new), h, d, dtype) for h in (heads, kv, kv))
+    gone = slice(new[0], new[0] + new[1])
+    q[gone] = k[gone] = v[gone] = float("nan")
+    kept = [i for i in range(sum(new)) if not gone.start <= i < gone.stop]
+    out, turned, mine = torch.full_like(q, 3.0), torch.full_like(q, 5.0), pool.clone()
+    tt.paged_append(k, v, mine[0], mine[1], table, cu, lens, q=q, freqs=freqs, out=turned, room=room)
+    tt.paged_attention(turned, mine[0], mine[1], table, cu, lens, out=out, room=room)
+    assert status() == _capi.OK
+    assert (turned[gone] == 5.0).all() and (out[gone] == 3.0).all()
+    # the same call without them
+    two, cu2 = [0, 2], cumulative([new[0], new[2]])
+    want_q = tt.paged_append(k[kept], v[kept], pool[0], pool[1], table[two], cu2, lens[two], q=q[kept], freqs=freqs)
+    want = tt.paged_attention(want_q, pool[0], pool[1], table[two], cu2, lens[two])
+    assert status() == _capi.OK and torch.equal(mine, pool) and torch.equal(turned[kept], want_q)
+    # dealt out otherwise: each may be off by half a step of itself and half a step of each probability, 2^-14 for everything in fp32
+    u = torch.finfo(dtype).eps / 2
+    off = 2 * (u * want.abs().max() + (u + 2.0 ** -14) * pool[1].abs().max()).item()
+    assert (out[kept].double() - want.double()).abs().max() <= off
+
+
+def test_refused_rows_of_a_full_pool_stay_as_they_are_and_go_on_later():
+    """Two beams share a begun page and nothing is free: neither writes to it, their lengths and tables stay; when a third request ends they go on, each in a page of its own."""
+    kv, d, page, dtype = 2, 64, 16, torch.float16
+    cache = tt.PagedKVCache(1, 4, 4, 64, kv, d, page, dtype, DEV)
+    g = torch.Generator(DEV).manual_seed(0)
+    cache.pool.zero_()
+
+    def play(new):
+        granted = cache.reserve(new).tolist()
+        k, v = rows(g, sum(new), kv, d, dtype), rows(g, sum(new), kv, d, dtype)
+        cu = cumulative(new)
+        cache.append(0, k, v, cu)
+        out = cache.attend(0, rows(g, sum(new), kv, d, dtype), cu)
+        cache.advance(new)
+        return granted, out
+
+    assert play([10, 0, 32, 0])[0] == [1] * 4
+    cache.fork([0, 0, 2, 3])  # the pool: one page shared by two, two of the third, one free
+    assert play([0, 0, 0, 5])[0] == [1] * 4
+    before = [x.clone() for x in (cache.table, cache.lens, cache.refs, cache.pool)]
+    assert cache.refs.tolist() == [2, 1, 1, 1]
+    for new in ([1, 1, 0, 0], [1, 0, 0, 0], [0, 20, 0, 1], [1, 1, 64, 0]):
+        granted, _ = play(new)
+        assert granted == [int(n == 0) for n in new] and cache.room.tolist() == granted
+        assert all(torch.equal(a, b) for a, b in zip(before, (cache.table, cache.lens, cache.refs, cache.pool)))
+    assert status() == _capi.OK
+    cache.release([2])
+    granted, out = play([1, 1, 0, 3])
+    assert granted == [1] * 4 and cache.lens.tolist() == [11, 11, 0, 8] and status() == _capi.OK and out.isfinite().all()
+    assert cache.refs.tolist() == [1, 1, 0, 1] and cache.table[:, 0].tolist() == [1, 0, -1, 3]
+    assert torch.equal(cache.pool[:, 1, :, :10], before[3][:, 0, :, :10]) and torch.equal(cache.pool[:, 0, :, :10], before[3][:, 0, :, :10])
+    cache.release(range(4))
+    assert (cache.refs == 0).all() and (cache.lens == 0).all()
+
+
+def test_a_captured_step_goes_by_what_is_granted_when_it_is_replayed():
+    """A pool that fills up while a captured step is replayed: the rows stop in their order and go on after one of them is freed, as in the eager run beside it."""
+    B, kv, d, page, dtype = 4, 2, 64, 16, torch.bfloat16
+    g = torch.Generator(DEV).manual_seed(3)
+    q, k, v = (rows(g, B, kv, d, dtype) for _ in range(3))
+    cu, ones = cumulative([1] * B), ints([1] * B)
+
+    def step(c, out):
+        c.reserve(ones)
+        c.append(0, k, v, cu)
+        c.attend(0, q, cu, out=out)
+        c.advance(ones)
+
+    eager, captured = (tt.PagedKVCache(1, 6, B, 160, kv, d, page, dtype, DEV) for _ in range(2))
+    for c in (eager, captured):
+        c.pool.zero_()
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    step(tt.PagedKVCache(1, 6, B, 160, kv, d, page, dtype, DEV), torch.zeros_like(q))  # (a first run loads the kernels, which a capture should not)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    cxx.arena_begin(0, 64 << 20)
+    with torch.cuda.graph(graph, stream=side):
+        step(captured, outs[1])
+    arena = cxx.arena_end(0)[1]
+    cxx.set_stream(0, torch.cuda.current_stream().cuda_stream)
+    seen = set()
+    for i in range(60):
+        step(eager, outs[0])
+        graph.replay()
+        if i == 45:
+            for c in (eager, captured):
+                c.release([1])
+        torch.cuda.synchronize()
+        seen.add(tuple(eager.room.tolist()))
+        for a, b in zip((eager.table, eager.lens, eager.refs, eager.room, outs[0]), (captured.table, captured.lens, captured.refs, captured.room, outs[1])):
+            assert torch.equal(a, b)
+    assert (1, 1, 1, 1) in seen and (1, 1, 0, 0) in seen and (0, 0, 0, 0) in seen and status() == _capi.OK
+    del graph
+    cxx.arena_release(0, arena)

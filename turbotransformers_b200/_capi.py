@@ -61,7 +61,7 @@ class RotaryArgs(C.Structure):
 class PagedKV(C.Structure):
     """ttb_paged_kv of include/ttb.h."""
     _fields_ = [("keys", p), ("values", p)] + [(n, i64) for n in ("page_stride", "pages", "kv_heads", "page_tokens", "d")] + \
-               [("table", p), ("table_stride", i64), ("table_width", i64), ("cu_seqlens", p), ("past_lens", p), ("B", i64)]
+               [("table", p), ("table_stride", i64), ("table_width", i64), ("cu_seqlens", p), ("past_lens", p), ("B", i64), ("room", p)]
 
 
 class PagedRotary(C.Structure):
@@ -71,7 +71,7 @@ class PagedRotary(C.Structure):
 
 class PagedTables(C.Structure):
     """ttb_paged_tables of include/ttb.h."""
-    _fields_ = [("table", p), ("stride", i64), ("B", i64), ("width", i64), ("lens", p), ("refs", p), ("pages", i64)]
+    _fields_ = [("table", p), ("stride", i64), ("B", i64), ("width", i64), ("lens", p), ("refs", p), ("pages", i64), ("room", p)]
 
 
 class PagedPool(C.Structure):

@@ -34,6 +34,7 @@ struct RotaryParams {
   const int64_t* positions;
   const double* freqs;
   Sequences s;              // PAGED
+  const int32_t* room;      // may be null
   void *keys, *values;
   long long page_stride;
 };
@@ -147,7 +148,7 @@ __device__ __forceinline__ void block_angles(const RotaryParams& p, int t0, int 
     bool bad = false, mine = false;
     long long place = -1;
     int at = 0;
-    if (b >= 0 && b < p.s.B) {
+    if (b >= 0 && b < p.s.B && !(p.room && p.room[b] == 0)) {
       const Sequence q = sequence_of(p.s, b, &bad);
       mine = t >= q.tok0 && t < q.tok0 + q.n;
       at = q.past + t - q.tok0;
@@ -370,6 +371,7 @@ struct Tables {
   int B, width, pages;
   int32_t *lens, *refs;
   int* status;
+  int32_t* room;
 };
 
 // Pages for new[b] more tokens of every row (see ttb.h for the rules). One block; thread b decides for row b.
@@ -497,6 +499,7 @@ paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page
   const int c = block_scan(copy ? 1 : 0, scratch, &n_copies);
   if (b < t.B) {
     granted[b] = ok;
+    if (t.room) t.room[b] = ok;
     if (!ok) s_want[b] = first;  // nothing to fill in
     s_at[b] = before + own;
     if (copy) {
@@ -662,7 +665,7 @@ int check_tables(ttb_ctx* ctx, const char* what, const ttb_paged_tables* a, Tabl
   TTB_REQUIRE(ctx, a->B >= 0 && a->B <= kMaxSequences, "%s: at most %d rows", what, kMaxSequences);
   TTB_REQUIRE(ctx, a->width > 0 && a->width < (1ll << 30) && a->stride >= a->width, "%s: bad table width", what);
   TTB_REQUIRE(ctx, a->pages > 0 && a->pages < (1ll << 30), "%s: bad number of pages", what);
-  *t = Tables{a->table, a->stride, (int)a->B, (int)a->width, (int)a->pages, a->lens, a->refs, ctx->d_status};
+  *t = Tables{a->table, a->stride, (int)a->B, (int)a->width, (int)a->pages, a->lens, a->refs, ctx->d_status, a->room};
   return TTB_OK;
 }
 
@@ -743,6 +746,7 @@ extern "C" int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv,
   DeviceGuard g(ctx->device);
   p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
   p.keys = kv->keys; p.values = kv->values; p.page_stride = kv->page_stride;
+  p.room = kv->room;
   p.tokens = (int)tokens;
   return dtype == TTB_F16 ? launch_rotary<__half, true>(ctx, p, "paged_append") : launch_rotary<__nv_bfloat16, true>(ctx, p, "paged_append");
 }

@@ -647,6 +647,7 @@ extern "C" int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* 
   p.ldo = ldo;
   p.group = (int)(heads / kv->kv_heads);
   p.scale = scale * kLog2e;
+  p.room = kv->room;
   p.split.causal = causal != 0;
   if (kv->d == 64) return dtype == TTB_F16 ? launch_all<__half, 64>(ctx, dtype, kv, heads, p) : launch_all<__nv_bfloat16, 64>(ctx, dtype, kv, heads, p);
   return dtype == TTB_F16 ? launch_all<__half, 128>(ctx, dtype, kv, heads, p) : launch_all<__nv_bfloat16, 128>(ctx, dtype, kv, heads, p);

@@ -34,6 +34,7 @@ struct Params {
   int group;      // query heads of a key head
   int low, high;  // the kernel takes the sequences of low to high new tokens
   float scale;    // times log2 e
+  const int32_t* room;  // may be null
   Parts parts;
 };
 
@@ -51,9 +52,13 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
   __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
-// Sequence b, without new tokens where it is the other kernel's.
+// Sequence b, without new tokens where it is the other kernel's, or passed over for want of room.
 __device__ __forceinline__ Sequence taken(const Params& p, int b, bool* bad) {
   Sequence q = sequence_of(p.s, b, bad);
+  if (p.room && p.room[b] == 0) {
+    q.n = 0;
+    *bad = false;
+  }
   if (q.n < p.low || q.n > p.high) q.n = 0;
   return q;
 }

@@ -6,12 +6,15 @@ frequencies of rotary positions. One step of a batch whose sequence b has new[b]
 
     cache = PagedKVCache(layers=24, pages=20000, sequences=64, max_tokens=4096, kv_heads=8, head_size=128)
     rotary = RotaryEmbedding(128, device="cuda")
-    granted = cache.reserve(new)                           # pages for the new tokens (int32 [64] on the device)
+    granted = cache.reserve(new)                           # pages for the new tokens: int32 [64] on the device, 0 where there were none
     for layer in ...:
         q = cache.append(layer, k, v, cu_seqlens, q=q, rotary=rotary)
         context = cache.attend(layer, q, cu_seqlens)       # [tokens, heads, head_size]
-    cache.advance(new)
+    cache.advance(new)                                     # of the rows that were granted
     cache.fork(parents)                                    # beams follow their parents; -1 frees a row
+
+A row that was not granted stays as it was: append and attend pass it over (its rows of their outputs are undefined), advance does not count its tokens, and it can
+ask again when others have been freed.
 
 Nothing here waits for the device or reads from it, so that a step can be captured into a graph; what an index outside its table comes to is said in
 include/ttb.h, and device_status reports it. The reference has no counterpart: its decoder concatenates one cache of equally long sequences a step
@@ -84,7 +87,7 @@ def _table(table, device):
     return table.data_ptr(), row if B > 1 else width, B, width
 
 
-def _kv(keys, values, table, cu_seqlens, past_lens, dtype, device):
+def _kv(keys, values, table, cu_seqlens, past_lens, room, dtype, device):
     """The arguments that describe one layer's pages."""
     shape, strides = keys.shape, keys.stride()
     if len(shape) != 4 or shape != values.shape:
@@ -96,7 +99,8 @@ def _kv(keys, values, table, cu_seqlens, past_lens, dtype, device):
         _fail("keys and values", "must have contiguous pages, equally far apart")
     at, row, B, width = _table(table, device)
     return (keys.data_ptr(), values.data_ptr(), strides[0] if pages > 1 else heads * tokens * d, pages, heads, tokens, d, at, row, width,
-            _index(cu_seqlens, "cu_seqlens", B + 1, device), _index(past_lens, "past_lens", B, device), B)
+            _index(cu_seqlens, "cu_seqlens", B + 1, device), _index(past_lens, "past_lens", B, device), B,
+            0 if room is None else _index(room, "room", B, device))
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, freqs: torch.Tensor, *, interleaved: bool = False, scale: float = 1.0,
@@ -131,10 +135,11 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor,
                  past_lens: torch.Tensor, *, q: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None, interleaved: bool = False, scale: float = 1.0,
-                 out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+                 out: Optional[torch.Tensor] = None, room: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Files k and v [tokens, key heads, d] of new tokens as tokens past_lens[b] and following of their sequences. Sequence b's are rows cu_seqlens[b] to
     cu_seqlens[b + 1]; table int32 [sequences, width] lists the pages of each; keys and values are the layer's pool [pages, key heads, page tokens, d]. With `freqs` (see
-    rotary) the keys are turned by their places on the way, and so is q, which is returned in a new tensor or in `out`."""
+    rotary) the keys are turned by their places on the way, and so is q, which is returned in a new tensor or in `out`. Sequences with 0 in room (int32 [sequences],
+    what paged_reserve granted) are passed over: nothing of them is filed, and their rows of q are not turned."""
     device, dtype = _gpu(k, "k"), k.dtype
     if dtype not in _CODE:
         _fail("k", "must be fp16 or bf16")
@@ -142,7 +147,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: t
     n, other, _, ldv = _rows(v, "v", device, dtype, d)
     if n != T or other != heads:
         _fail("v", "must be like k")
-    kv = _kv(keys, values, table, cu_seqlens, past_lens, dtype, device)
+    kv = _kv(keys, values, table, cu_seqlens, past_lens, room, dtype, device)
     if kv[4] != heads or kv[6] != d:
         _fail("k", "must have the pool's heads")
     if freqs is None:
@@ -166,15 +171,16 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, keys: torch.Tensor, values: t
 
 
 def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, table: torch.Tensor, cu_seqlens: torch.Tensor, past_lens: torch.Tensor, *,
-                    causal: bool = True, scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    causal: bool = True, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    room: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of q [tokens, heads, d] over the pages of its sequences (arguments as for paged_append, whose new tokens have been filed): token i of a sequence sees its
-    cached tokens up to itself, or all past + new of them if not causal. heads is a multiple of the key heads; scale is d ** -0.5 unless given. Rows that belong to no sequence
-    are left as they are in `out`, undefined without it."""
+    cached tokens up to itself, or all past + new of them if not causal. heads is a multiple of the key heads; scale is d ** -0.5 unless given. Rows that belong to no sequence,
+    or to one with 0 in room (as for paged_append), are left as they are in `out`, undefined without it."""
     device, dtype = _gpu(q, "q"), q.dtype
     if dtype not in _CODE:
         _fail("q", "must be fp16 or bf16")
     T, heads, d, ldq = _rows(q, "q", device, dtype)
-    kv = _kv(keys, values, table, cu_seqlens, past_lens, dtype, device)
+    kv = _kv(keys, values, table, cu_seqlens, past_lens, room, dtype, device)
     if kv[6] != d or heads % max(kv[4], 1):
         _fail("q", "must have the pool's head size, and a multiple of its heads")
     if out is None:
@@ -208,14 +214,15 @@ def _pool(pool):
     return pool.data_ptr(), planes, size * (strides[0] if planes > 1 else pages * page_stride), pages, size * page_stride, size * page
 
 
-def paged_reserve(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, new_tokens: torch.Tensor, page_tokens: int):
+def paged_reserve(table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, new_tokens: torch.Tensor, page_tokens: int, *, room: Optional[torch.Tensor] = None):
     """Room for new_tokens[b] more tokens of every row of the page table: pages that the row lists already behind its tokens, then the lowest free ones (those of refs 0),
     which are taken into the table. A row that would write to a page that other rows list too gets one of its own in its place. Returns (granted int32 [sequences], copies int32 [sequences, 2]); hand the copies to paged_copy before the new
-    tokens are filed. A row that is not granted (0) has been left alone: the pool is full, or its row of the table, or the row or its number of tokens is bad (see device_status)."""
+    tokens are filed. A row that is not granted (0) has been left alone: the pool is full, or its row of the table, or the row or its number of tokens is bad (see device_status).
+    room (int32 [sequences]) receives what is granted too: a tensor that is kept from step to step, for paged_append and paged_attention."""
     device, t = _tables(table, lens, refs)
     new = _index(new_tokens, "new_tokens", t[2], device)
     granted, copies = torch.empty_like(new_tokens), new_tokens.new_empty((t[2], 2))
-    cxx.paged_reserve(device, _stream(device), *t, new, page_tokens, granted.data_ptr(), copies.data_ptr())
+    cxx.paged_reserve(device, _stream(device), *t, new, page_tokens, granted.data_ptr(), copies.data_ptr(), 0 if room is None else _index(room, "room", t[2], device))
     return granted, copies
 
 
@@ -284,7 +291,8 @@ class RotaryEmbedding:
 
 class PagedKVCache:
     """The keys and values of a stack of layers in one pool of pages, and the sequences that they belong to. Row b of the page table is sequence b: `sequences` of them at once,
-    a row without tokens being free. `lens` (int32, on the device) are the tokens cached; advance() moves them on when all layers have filed a step's tokens."""
+    a row without tokens being free. `lens` (int32, on the device) are the tokens cached; advance() moves them on when all layers have filed a step's tokens. `room` (int32, on the
+    device) is what reserve() granted last, which append(), attend() and advance() go by: 1 for all rows before the first."""
 
     def __init__(self, layers: int, pages: int, sequences: int, max_tokens: int, kv_heads: int, head_size: int, page_tokens: int = 16,
                  dtype: torch.dtype = torch.float16, device: Union[str, torch.device] = "cuda"):
@@ -296,13 +304,14 @@ class PagedKVCache:
         self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(sequences, dtype=torch.int32, device=device)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self.room = torch.ones(sequences, dtype=torch.int32, device=device)
 
     def _counts(self, values) -> torch.Tensor:
         return values if isinstance(values, torch.Tensor) else torch.tensor(values, dtype=torch.int32).to(self.table.device)
 
     def reserve(self, new_tokens: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
         """Pages for new_tokens[b] more tokens of every sequence; pages that are shared and about to be written are copied. Returns what paged_reserve grants."""
-        granted, copies = paged_reserve(self.table, self.lens, self.refs, self._counts(new_tokens), self.page_tokens)
+        granted, copies = paged_reserve(self.table, self.lens, self.refs, self._counts(new_tokens), self.page_tokens, room=self.room)
         paged_copy(self.pool, copies)
         return granted
 
@@ -311,15 +320,16 @@ class PagedKVCache:
         turn = {} if rotary is None else {"q": q, "freqs": rotary.freqs, "interleaved": rotary.interleaved, "scale": rotary.scale, "out": out}
         if rotary is None and q is not None:
             raise ValueError("q is turned by rotary positions: it has none without them")
-        return paged_append(k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.table, cu_seqlens, self.lens, **turn)
+        return paged_append(k, v, self.pool[2 * layer], self.pool[2 * layer + 1], self.table, cu_seqlens, self.lens, room=self.room, **turn)
 
     def attend(self, layer: int, q, cu_seqlens, causal: bool = True, scale: Optional[float] = None, out=None):
         """paged_attention over a layer's pages, between append and advance."""
-        return paged_attention(q, self.pool[2 * layer], self.pool[2 * layer + 1], self.table, cu_seqlens, self.lens, causal=causal, scale=scale, out=out)
+        return paged_attention(q, self.pool[2 * layer], self.pool[2 * layer + 1], self.table, cu_seqlens, self.lens, causal=causal, scale=scale, out=out,
+                               room=self.room)
 
     def advance(self, new_tokens: Union[torch.Tensor, Sequence[int]]) -> None:
-        """The new tokens are cached now."""
-        self.lens += self._counts(new_tokens)
+        """The new tokens are cached now, those of the sequences that had room. Fewer than were reserved may be kept: the rest of the room stays the sequence's."""
+        self.lens.addcmul_(self._counts(new_tokens), self.room)
 
     def fork(self, parents: Union[torch.Tensor, Sequence[int]]) -> None:
         """paged_fork: sequence b becomes what parents[b] was; -1 frees it."""
