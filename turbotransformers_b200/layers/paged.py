@@ -72,8 +72,8 @@ def _index(t, name, n, device, dtype=torch.int32):
 
 
 def _freqs(freqs, device):
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or freqs.get_device() != device:
-        _fail("freqs", f"must be a contiguous float64 vector on cuda:{device}")
+    if freqs.dtype != torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or freqs.get_device() != device or freqs.shape[0] == 0:
+        _fail("freqs", f"must be a contiguous float64 vector on cuda:{device}, of one at least")
     return freqs.data_ptr(), 2 * freqs.shape[0]
 
 
