@@ -7,8 +7,8 @@
 // into the next tile; four take 32 keys each of every unit, with a softmax state of their own, and join the four states at the tile's end. Their products are
 // mma.sync m16n8k16 with the keys as rows: a tile of eight queries fills it, where the tensor memory's 128 rows would be empty but for eight. Parts of a tile that was cut
 // go to a workspace in fp32 and a second kernel joins them, in the order of the keys.
-// A row's reference is the maximum of its first keys, raised (and its sums rescaled) only where the probabilities of 32 keys sum to more than 2^15; the division by the sum
-// makes the result independent of it. Scores, references and sums are fp32; the probabilities are rounded to the values' 16 bits, the only form in which the
+// A row's reference is the maximum of its first keys (fp16: 2^6 below it), raised (and its sums rescaled) only where four probabilities, a lane's, sum to 2^15 and more; the division by
+// the sum makes the result independent of it. Scores, references and sums are fp32; the probabilities are rounded to the values' 16 bits, the only form in which the
 // tensor cores take both (half a step of each, of both signs, against a sum of them that is not rounded).
 // 64 requests of 20 to 4000 tokens, 12 heads of 64, fp16: 89 us, 5.1 TB/s (110 with one loading warp and 16-row tiles throughout). One token over 8000, 32 heads of
 // 128 on 8 key heads, bf16: 15 us, of which 3 go by before the first load (the sequences, the part, its pages) and some 5 are the join and its launch.
@@ -329,8 +329,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 if (x * 8 >= limit) s[x >> 1][nt][(x & 1) * 2 + q] = -INFINITY;
             }
         }
-        // A row's reference is the maximum of its first keys; it is raised (and the sums rescaled) only where probabilities sum up to 2^15 and more: the division by
-        // the sum makes the result independent of it.
+        // A row's reference is the maximum of its first keys (fp16: 2^6 below it); it is raised (and the sums rescaled) only where a lane's four probabilities sum up to 2^15 and
+        // more: the division by the sum makes the result independent of it.
         uint32_t pf[2][NT][2];
         while (true) {
           if (fresh) {
@@ -338,7 +338,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int q = 0; q < 2; ++q) {
-                const float top = column_max(fmaxf(fmaxf(s[0][nt][q], s[0][nt][2 + q]), fmaxf(s[1][nt][q], s[1][nt][2 + q]))) * p.scale;
+                const float top = column_max(fmaxf(fmaxf(s[0][nt][q], s[0][nt][2 + q]), fmaxf(s[1][nt][q], s[1][nt][2 + q]))) * p.scale - kBelow<T>;
                 const float m_new = fmaxf(m[nt][q], top), corr = m_new == -INFINITY ? 1.f : ex2(m[nt][q] - m_new);
                 m[nt][q] = m_new;
                 l[nt][q] *= corr;

@@ -38,6 +38,13 @@ struct Params {
   Parts parts;
 };
 
+// How far below the maximum of its first keys a row's reference lies (log2). fp16 has no normal numbers under 2^-14: where one key outweighs each of thousands of others by that much, as
+// the first of a text may, every one of theirs would be rounded to a multiple of 2^-24 (17 above them: to 1.4 times itself). So the largest probabilities are 2^6 and more,
+// and the edge lies at 2^-20 of them, half a step below it being 2^-31. More would bring sums of 128 equal ones to the limit of 2^15 at which a reference is raised.
+// bf16 has fp32's range.
+template <typename T> constexpr float kBelow = 0.f;
+template <> constexpr float kBelow<__half> = 6.f;
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -9,8 +9,9 @@
 //   warps 1, 3  : matrix products of a set each - S = Q K^T (128 x 128, fp32 in TMEM), O += P V with P in TMEM over the scores it came from, V as it lies, in
 //                 the order QK(0), PV(0), QK(1), PV(1), ...; everything a product waits for but the softmax is a barrier poll
 //   warps 4..11 : softmax, a warpgroup a set, a row a thread: scores from TMEM, exp2 with the scale folded in, P back to TMEM in 16 bits. The row's reference is the maximum of
-//                 its first 32 keys; it is raised (and O rescaled) only where the sum of 32 probabilities passes 2^15: the division by the sum makes the result independent of it. References
-//                 are whole numbers (of log2), so that probabilities that are brought to a new one are not rounded a second time.
+//                 its first 32 keys (fp16: 2^6 below it); it is raised (and O rescaled) only where the sum of 32 probabilities passes 2^15: the division by the sum makes the result
+//                 independent of it. References are whole numbers (of log2), so that probabilities that are brought to a new one are not rounded a second time (unless, in fp16,
+//                 they fall below 2^-14 there, 2^-20 of the largest).
 // A tile's output is written while the next one's first scores are made. Every wait is bounded. The probabilities are rounded to the values' 16 bits, as in the kernel for few
 // rows; their sums are not.
 // 4000 tokens over 12000, 32 heads of 128 on 8 key heads, bf16: 890 us, 1.03 PFLOP/s of products that the mask leaves; a pair of units takes 4400 cycles, of which the products
@@ -540,7 +541,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             float top = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 32; e += 2) top = fmaxf(fmaxf(top, __uint_as_float(r[e])), __uint_as_float(r[e + 1]));
-            m_used = floorf(top * p.scale);
+            m_used = floorf(top * p.scale) - kBelow<T>;
           }
           // A tile that every row sees the whole of: straight through, P kept until its sum says that the reference still holds. Short code, since the instruction cache is the other warps' too (with masks and rescaling in it 16 products took 3500 cycles in place of 1250).
           float l0 = 0.f, l1 = 0.f;
@@ -603,7 +604,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                   float top = -INFINITY;
 #pragma unroll
                   for (int e = 0; e < 32; ++e) top = fmaxf(top, x[e]);
-                  const float m_new = fmaxf(m_used, floorf(m_sub + top)), corr = m_new == -INFINITY ? 1.f : power_of_2(m_used - m_new);
+                  const float m_new = fmaxf(m_used, floorf(m_sub + top) - kBelow<T>), corr = m_new == -INFINITY ? 1.f : power_of_2(m_used - m_new);
                   const float down = m_sub - (m_new == -INFINITY ? 0.f : m_new);
                   m_used = m_new;
                   l_run *= corr;
