@@ -335,9 +335,9 @@ class PagedKVCache:
         """paged_fork: sequence b becomes what parents[b] was; -1 frees it."""
         paged_fork(self.table, self.lens, self.refs, self._counts(parents))
 
-    def release(self, sequences: Sequence[int]) -> None:
-        """Frees these sequences' pages (those that no other lists)."""
-        gone = set(sequences)
+    def release(self, sequences: Union[torch.Tensor, Sequence[int]]) -> None:
+        """Frees these sequences' pages (those that no other lists). (A tensor of them is read by the host; fork() takes parents on the device.)"""
+        gone = set(sequences.tolist() if isinstance(sequences, torch.Tensor) else sequences)
         self.fork([-1 if b in gone else b for b in range(self.table.shape[0])])
 
     def compact(self) -> torch.Tensor:
