@@ -450,7 +450,9 @@ int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t to
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the cached tokens of t's sequence up to and including its own (causal), or all past + new of them.
  * The new tokens have been filed (ttb_paged_append). q and out [tokens, heads, d], heads a multiple of kv_heads (query heads h * heads / kv_heads and
  * following share key head h), ldq / ldo elements between tokens (% 8 == 0), 16-byte aligned; out does not overlap q. scale > 0. What the pages hold behind a
- * sequence's last token is not looked at; the keys and values of its own tokens are to be finite. A page that is not in the pool is read as page 0. */
+ * sequence's last token is not looked at; the keys and values of its own tokens are to be finite. A page that is not in the pool is read as page 0. Parts of what is split over
+ * SMs go to a workspace of the context's pool: 2 * SMs * rows * d * 4 bytes, rows 256 where sequences may have many rows (heads of 128 on 148 SMs: 39 MB), 8 to 32 otherwise, and
+ * both where a call may have either. In an arena (a captured pass) every call has its own. */
 int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const void* q, int64_t ldq, int64_t tokens, int64_t heads, int causal, float scale,
                         void* out, int64_t ldo);
 

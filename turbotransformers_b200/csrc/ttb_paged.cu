@@ -16,8 +16,8 @@ namespace {
 // million times a frequency in fp32 would be off by a tenth of a radian. With a pool of pages, k is turned on its way into its page and v copied beside it: a pass
 // of its own over both, and a launch, saved. The rows are on their way while the block looks up its positions and pages.
 // 8000 tokens of 40 heads of 128, fp32, all of each turned: 59 us, 5.5 TB/s; 64 and 200 tokens of 40 heads of 128, 16 bits: 5 and 7 us, a chain of dependent reads.
-// Units of a thread, threads of an SM and units of a block were measured together: two, 1536 and 1024 (15000 tokens of 32 heads of 64, fp16, and 7900 of 48 of 128, with the launch: 31 and 47 us;
-// four units and 1024 threads 31 and 51; one unit and 512 to a block 31 to 43 and 49 to 63).
+// Units of a thread, threads of an SM and units of a block were measured together, at sizes that the kernel by heads below has taken over since: two, 1536 and 1024 (15000 tokens of 32 heads
+// of 64, fp16, and 7900 of 48 of 128, with the launch: 31 and 47 us; four units and 1024 threads 31 and 51; one unit and 512 to a block 31 to 43 and 49 to 63).
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryTokens = 8;  // of a block, at most
 constexpr int kRotaryUnits = 2;   // that a thread has on their way

@@ -572,7 +572,8 @@ template <typename T, int D>
 int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, Params& p) {
   // Which kernels, and the rows of a tile of the one for few. The host knows the sum of the new tokens only. With no more tokens than sequences, tiles of a token's rows (up to 32)
   // take all of them, a sequence of several tokens several tiles. Otherwise tiles of an average sequence's rows, up to 32 (24 with heads of
-  // 128), and the sequences that have more go to the kernel for many; where the average has more, tiles of 16. Rows of a sequence, us in tiles of 32 here and on the kernel for
+  // 128), and the sequences that have more go to the kernel for many; where the average has more, tiles of 16. Sequences without new tokens count: a table of many idle rows looks
+  // like one of single tokens, and a chunk among them is walked in small tiles (right, and slower). Rows of a sequence, us in tiles of 32 here and on the kernel for
   // many, with cold caches: 64 requests of 3 tokens over 500 to 4000, 24 rows, heads of 64 76 and 88, of 128 172 and 182; 100 of 8 over 100 to 1000, 32 rows, 68 and 70, 148 and
   // 130; 16 of 3 to 6 over up to 16000, 24 to 48 rows, 128: 171 and 144 to 151.
   const int64_t tokens = p.s.tokens, B = kv->B, each = (tokens + B - 1) / B * p.group;

@@ -165,7 +165,7 @@ __device__ __forceinline__ void next_part(const Params& p, Part& t, long long le
   fill_part(p, t, left);
 }
 
-// first query head of a head block, and how many of its rows per token exist (the last block of a key head may be short)
+// The first query head of a head block.
 __device__ __forceinline__ int first_head(const Params& p, int block) {
   return block / p.split.head_blocks * p.group + block % p.split.head_blocks * p.split.block_heads;
 }
@@ -227,7 +227,8 @@ inline bool encode_maps(const ttb_paged_kv* kv, bool bf16, int64_t heads, const 
          sm100::encode_tile_map_3d(v, kv->values, bf16, pages, rows, d, stride, d, 1, box_rows);
 }
 
-// The kernel for many rows (ttb_paged_attention_tc.cu) on tiles of kManyRows: launches it, parts of cut tiles going to p.parts.
+// The kernel for many rows (ttb_paged_attention_tc.cu) on tiles of kManyRows: launches it, parts of cut tiles going to p.parts (39 MB with heads of 128 and 148 SMs, whatever the
+// call: lengths are not known here).
 int paged_tc_launch(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, const Params& p);
 
 }  // namespace paged

@@ -18,7 +18,8 @@ namespace paged {
 
 constexpr int kMaxSequences = 1024;  // of a call: their places in the line are kept in shared memory
 
-// sum of floor((a * i + b) / m) for i < n, all of them not negative, m > 0: the lattice points under a line, by the steps of Euclid's algorithm
+// sum of floor((a * i + b) / m) for i < n, all of them not negative, m > 0: the lattice points under a line. Whole multiples of m come out of a and b; of what is left rows and
+// columns of the points change places, which changes a and m as a step of Euclid's algorithm does (Graham, Knuth and Patashnik, Concrete Mathematics, 3.5, floor sums)
 TTB_PAGED_FN int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
   int64_t sum = 0;
   while (n > 0) {

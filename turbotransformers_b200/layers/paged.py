@@ -16,8 +16,9 @@ frequencies of rotary positions. One step of a batch whose sequence b has new[b]
 A row that was not granted stays as it was: append and attend pass it over (its rows of their outputs are undefined), advance does not count its tokens, and it can
 ask again when others have been freed.
 
-Nothing here waits for the device or reads from it, so that a step can be captured into a graph; what an index outside its table comes to is said in
-include/ttb.h, and device_status reports it. The reference has no counterpart: its decoder concatenates one cache of equally long sequences a step
+Nothing here reads from the device, and with numbers of tokens and parents in int32 tensors nothing waits for it, so that a step can be captured into a graph; those given
+as Python lists are copied there first, which waits. What an index outside its table comes to is said in include/ttb.h, and device_status reports it. It is a serving
+path: results carry no gradient, as those of the other layers do not. The reference has no counterpart: its decoder concatenates one cache of equally long sequences a step
 (multi_headed_attention.cpp:207-231).
 """
 import math
@@ -174,7 +175,7 @@ def paged_attention(q: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, t
                     causal: bool = True, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                     room: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of q [tokens, heads, d] over the pages of its sequences (arguments as for paged_append, whose new tokens have been filed): token i of a sequence sees its
-    cached tokens up to itself, or all past + new of them if not causal. heads is a multiple of the key heads; scale is d ** -0.5 unless given. Rows that belong to no sequence,
+    cached tokens up to itself, or all past + new of them if not causal. heads is a multiple of the key heads; scale is d ** -0.5 unless given. out does not overlap q. Rows that belong to no sequence,
     or to one with 0 in room (as for paged_append), are left as they are in `out`, undefined without it."""
     device, dtype = _gpu(q, "q"), q.dtype
     if dtype not in _CODE:
