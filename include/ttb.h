@@ -420,9 +420,7 @@ int ttb_rotary(ttb_ctx* ctx, const ttb_rotary_args* args);
  *                  256; d 64 or 128
  *   table        : int32 [B, table_width], table_stride between rows: token j of sequence b is in page table[b][j / page_tokens], row j % page_tokens
  *   cu_seqlens   : int32 [B+1]: sequence b's new tokens are rows [cu[b], cu[b+1]) of the call's q, k, v; rows outside [cu[0], cu[B]) are left alone
- *   past_lens    : int32 [B]: tokens of sequence b that were cached before: new token i is token past + i
- *   room         : int32 [B] or NULL: sequences with 0 are passed over, as if they had no new tokens: nothing is filed, and their rows of the outputs are left alone
- *                  (ttb_paged_reserve's granted, so that a row without pages does no harm and the others go on) */
+ *   past_lens    : int32 [B]: tokens of sequence b that were cached before: new token i is token past + i */
 typedef struct ttb_paged_kv {
   void *keys, *values;
   int64_t page_stride, pages, kv_heads, page_tokens, d;
@@ -430,7 +428,6 @@ typedef struct ttb_paged_kv {
   int64_t table_stride, table_width;
   const int32_t *cu_seqlens, *past_lens;
   int64_t B;
-  const int32_t* room;
 } ttb_paged_kv;
 /* The rotary positions of ttb_paged_append: k is turned by its tokens' places in their sequences, and so is q[tokens, heads, d] into q_out (heads = 0: none). */
 typedef struct ttb_paged_rotary {
@@ -446,6 +443,10 @@ typedef struct ttb_paged_rotary {
  * not in the pool is not filed. No two rows of the table may list the same page where new tokens go. */
 int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv,
                      const ttb_paged_rotary* rotary);
+/* The same, and ttb_paged_attention below, of the sequences that have room: those with 0 in room (int32 [B] on the device, what ttb_paged_reserve granted) are passed over, as
+ * if they had no new tokens: nothing of them is filed, and their rows of the outputs are left alone. A row without pages does no harm, and the others go on. */
+int ttb_paged_append_room(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                          const ttb_paged_rotary* rotary, const int32_t* room);
 
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the cached tokens of t's sequence up to and including its own (causal), or all past + new of them.
  * The new tokens have been filed (ttb_paged_append). q and out [tokens, heads, d], heads a multiple of kv_heads (query heads h * heads / kv_heads and
@@ -455,16 +456,16 @@ int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t to
  * both where a call may have either. In an arena (a captured pass) every call has its own. */
 int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const void* q, int64_t ldq, int64_t tokens, int64_t heads, int causal, float scale,
                         void* out, int64_t ldo);
+int ttb_paged_attention_room(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const void* q, int64_t ldq, int64_t tokens, int64_t heads, int causal, float scale,
+                             void* out, int64_t ldo, const int32_t* room);
 
 /* The pages of B sequences: table int32 [B, width] (stride between rows), -1 behind a row's last page; lens int32 [B], the tokens cached; refs int32 [pages], how
- * many rows list a page (0: it is free). B * width < 2^31. room int32 [B] or NULL: receives
- * what ttb_paged_reserve grants as well, a place that stays while `granted` may be another's every step. */
+ * many rows list a page (0: it is free). B * width < 2^31. */
 typedef struct ttb_paged_tables {
   int32_t* table;
   int64_t stride, B, width;
   int32_t *lens, *refs;
   int64_t pages;
-  int32_t* room;
 } ttb_paged_tables;
 /* A stack's pages: `planes` (of each layer the keys and the values) of `pages` pages of page_bytes; strides in bytes; everything a multiple of 16. */
 typedef struct ttb_paged_pool {
@@ -480,6 +481,8 @@ typedef struct ttb_paged_pool {
  * (a length that the table cannot hold or a negative number of new tokens, which are TTB_ERR_BAD_INDEX, as is a row without a page for its last token). lens is left
  * to the caller, who adds the new tokens that were granted when all layers have filed them. */
 int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies);
+/* The same; room (int32 [B]) receives what is granted too: a place that stays, where `granted` may be another one every step. */
+int ttb_paged_reserve_room(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies, int32_t* room);
 /* Row b becomes what row parents[b] was (its pages are shared, not copied), for beams that follow their parents and requests that fork; -1 frees the row: its
  * length becomes 0. Any number of rows may have the same parent. A parent outside [-1, B) leaves its row as it is. */
 int ttb_paged_fork(ttb_ctx* ctx, const ttb_paged_tables* tables, const int32_t* parents);

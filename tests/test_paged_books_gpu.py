@@ -288,3 +288,29 @@ def test_a_captured_step_goes_by_what_is_granted_when_it_is_replayed():
     assert (1, 1, 1, 1) in seen and (1, 1, 0, 0) in seen and (0, 0, 0, 0) in seen and status() == _capi.OK
     del graph
     cxx.arena_release(0, arena)
+
+
+def test_room_through_the_c_interface(ctx):
+    """A step of three sequences of which the pool has room for the first: the same entry points with room, without it all rows as before."""
+    kv_heads, d, page, dtype = 2, 64, 16, torch.float16
+    g = torch.Generator(DEV).manual_seed(8)
+    table, lens, refs = ints([[2, -1], [0, -1], [3, -1]]), ints([16, 16, 3]), ints([1, 0, 1, 1])
+    granted, room, copies, new = ints([7] * 3), ints([7] * 3), ints([[7, 7]] * 3), ints([1, 1, 1])
+    ctx.paged_reserve(dict(table=table, stride=2, B=3, width=2, lens=lens, refs=refs, pages=4), new, page, granted, copies, room=room)
+    assert granted.tolist() == room.tolist() == [1, 0, 0] and table.tolist() == [[2, 1], [0, -1], [3, -1]]
+    pool = torch.randn(2, 4, kv_heads, page, d, generator=g, device=DEV, dtype=dtype)
+    q, k, v = (rows(g, 3, kv_heads, d, dtype) for _ in range(3))
+    kv = dict(keys=pool[0], values=pool[1], page_stride=pool.stride(1), pages=4, kv_heads=kv_heads, page_tokens=page, d=d, table=table, table_stride=2, table_width=2,
+              cu_seqlens=ints([0, 1, 2, 3]), past_lens=lens, B=3)
+    want, out = pool.clone(), torch.full_like(q, 3.0)
+    ctx.paged_append(_capi.F16, kv, 3, k, 128, v, 128, room=room)
+    want[0, 1, :, 0], want[1, 1, :, 0] = k[0], v[0]
+    assert torch.equal(pool, want)
+    ctx.paged_attention(_capi.F16, kv, q, 128, 3, kv_heads, 1, 0.125, out, 128, room=room)
+    assert ctx.device_status() == _capi.OK and (out[1:] == 3.0).all()
+    everything = torch.empty_like(q)
+    ctx.paged_attention(_capi.F16, {**kv, "table": ints([[2, 1], [0, 0], [3, 3]])}, q, 128, 3, kv_heads, 1, 0.125, everything, 128)
+    assert ctx.device_status() == _capi.OK and everything.isfinite().all()
+    # dealt out otherwise: each may be off by half a step of itself and half a step of each probability, 2^-14 for everything in fp32
+    u = torch.finfo(dtype).eps / 2
+    assert (everything[0].double() - out[0].double()).abs().max() <= 2 * (u * out[0].abs().max() + (u + 2.0 ** -14) * pool[1].abs().max()).item()

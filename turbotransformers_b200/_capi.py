@@ -61,7 +61,7 @@ class RotaryArgs(C.Structure):
 class PagedKV(C.Structure):
     """ttb_paged_kv of include/ttb.h."""
     _fields_ = [("keys", p), ("values", p)] + [(n, i64) for n in ("page_stride", "pages", "kv_heads", "page_tokens", "d")] + \
-               [("table", p), ("table_stride", i64), ("table_width", i64), ("cu_seqlens", p), ("past_lens", p), ("B", i64), ("room", p)]
+               [("table", p), ("table_stride", i64), ("table_width", i64), ("cu_seqlens", p), ("past_lens", p), ("B", i64)]
 
 
 class PagedRotary(C.Structure):
@@ -71,7 +71,7 @@ class PagedRotary(C.Structure):
 
 class PagedTables(C.Structure):
     """ttb_paged_tables of include/ttb.h."""
-    _fields_ = [("table", p), ("stride", i64), ("B", i64), ("width", i64), ("lens", p), ("refs", p), ("pages", i64), ("room", p)]
+    _fields_ = [("table", p), ("stride", i64), ("B", i64), ("width", i64), ("lens", p), ("refs", p), ("pages", i64)]
 
 
 class PagedPool(C.Structure):
@@ -113,7 +113,10 @@ SIGNATURES = {
     "ttb_rotary": (i32, [p, C.POINTER(RotaryArgs)]),
     "ttb_paged_append": (i32, [p, i32, C.POINTER(PagedKV), i64, p, i64, p, i64, C.POINTER(PagedRotary)]),
     "ttb_paged_attention": (i32, [p, i32, C.POINTER(PagedKV), p, i64, i64, i64, i32, f32, p, i64]),
+    "ttb_paged_append_room": (i32, [p, i32, C.POINTER(PagedKV), i64, p, i64, p, i64, C.POINTER(PagedRotary), p]),
+    "ttb_paged_attention_room": (i32, [p, i32, C.POINTER(PagedKV), p, i64, i64, i64, i32, f32, p, i64, p]),
     "ttb_paged_reserve": (i32, [p, C.POINTER(PagedTables), p, i64, p, p]),
+    "ttb_paged_reserve_room": (i32, [p, C.POINTER(PagedTables), p, i64, p, p, p]),
     "ttb_paged_fork": (i32, [p, C.POINTER(PagedTables), p]),
     "ttb_paged_copy": (i32, [p, C.POINTER(PagedPool), p, i64]),
     "ttb_paged_compact": (i32, [p, C.POINTER(PagedTables), C.POINTER(PagedPool), p]),
@@ -259,18 +262,25 @@ class Context:
         """ttb_rotary with the argument block filled by the fields' names; tensors are passed as their pointers, here and below."""
         self.check(lib().ttb_rotary(self.h, C.byref(self._filled(RotaryArgs(), fields))))
 
-    def paged_append(self, dtype, kv, tokens, k, ldk, v, ldv, rotary=None):
-        """ttb_paged_append; kv and rotary: dicts of their blocks' fields."""
+    def _with_room(self, name, room, *args):
+        """The entry point `name`, or its form that takes the sequences' room."""
+        if room is None:
+            self.check(getattr(lib(), name)(self.h, *args))
+        else:
+            self.check(getattr(lib(), name + "_room")(self.h, *args, p(room.data_ptr())))
+
+    def paged_append(self, dtype, kv, tokens, k, ldk, v, ldv, rotary=None, room=None):
+        """ttb_paged_append, or ttb_paged_append_room; kv and rotary: dicts of their blocks' fields."""
         block = C.byref(self._filled(PagedRotary(), rotary)) if rotary is not None else None
-        self.check(lib().ttb_paged_append(self.h, dtype, C.byref(self._filled(PagedKV(), kv)), tokens, p(k.data_ptr()), ldk, p(v.data_ptr()), ldv, block))
+        self._with_room("ttb_paged_append", room, dtype, C.byref(self._filled(PagedKV(), kv)), tokens, p(k.data_ptr()), ldk, p(v.data_ptr()), ldv, block)
 
-    def paged_attention(self, dtype, kv, q, ldq, tokens, heads, causal, scale, out, ldo):
-        self.check(lib().ttb_paged_attention(self.h, dtype, C.byref(self._filled(PagedKV(), kv)), p(q.data_ptr()), ldq, tokens, heads, causal, scale,
-                                             p(out.data_ptr()), ldo))
+    def paged_attention(self, dtype, kv, q, ldq, tokens, heads, causal, scale, out, ldo, room=None):
+        self._with_room("ttb_paged_attention", room, dtype, C.byref(self._filled(PagedKV(), kv)), p(q.data_ptr()), ldq, tokens, heads, causal, scale,
+                        p(out.data_ptr()), ldo)
 
-    def paged_reserve(self, tables, new_tokens, page_tokens, granted, copies):
-        self.check(lib().ttb_paged_reserve(self.h, C.byref(self._filled(PagedTables(), tables)), p(new_tokens.data_ptr()), page_tokens, p(granted.data_ptr()),
-                                           p(copies.data_ptr())))
+    def paged_reserve(self, tables, new_tokens, page_tokens, granted, copies, room=None):
+        self._with_room("ttb_paged_reserve", room, C.byref(self._filled(PagedTables(), tables)), p(new_tokens.data_ptr()), page_tokens, p(granted.data_ptr()),
+                        p(copies.data_ptr()))
 
     def paged_fork(self, tables, parents):
         self.check(lib().ttb_paged_fork(self.h, C.byref(self._filled(PagedTables(), tables)), p(parents.data_ptr())))

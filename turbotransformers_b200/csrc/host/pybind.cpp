@@ -78,8 +78,8 @@ ttb_ctx* OnStream(int device, Ptr stream) {
   return core::DeviceContext(device);
 }
 ttb_paged_kv KV(Ptr keys, Ptr values, int64_t page_stride, int64_t pages, int64_t kv_heads, int64_t page_tokens, int64_t d, Ptr table, int64_t table_stride,
-                int64_t table_width, Ptr cu, Ptr past, int64_t B, Ptr room) {
-  return {At(keys), At(values), page_stride, pages, kv_heads, page_tokens, d, Ints(table), table_stride, table_width, Ints(cu), Ints(past), B, Ints(room)};
+                int64_t table_width, Ptr cu, Ptr past, int64_t B) {
+  return {At(keys), At(values), page_stride, pages, kv_heads, page_tokens, d, Ints(table), table_stride, table_width, Ints(cu), Ints(past), B};
 }
 
 void Rotary(int device, Ptr stream, int dtype, Ptr q, Ptr k, Ptr q_out, Ptr k_out, int64_t ldq, int64_t ldk, int64_t ldq_out, int64_t ldk_out, int64_t tokens,
@@ -94,29 +94,29 @@ void PagedAppend(int device, Ptr stream, int dtype, Ptr keys, Ptr values, int64_
                  Ptr table, int64_t table_stride, int64_t table_width, Ptr cu, Ptr past, int64_t B, Ptr room, int64_t tokens, Ptr k, int64_t ldk, Ptr v, int64_t ldv, Ptr freqs,
                  int64_t rotary_dim, bool interleaved, float scale, Ptr q, Ptr q_out, int64_t ldq, int64_t ldq_out, int64_t heads) {
   ttb_ctx* c = OnStream(device, stream);
-  const ttb_paged_kv kv = KV(keys, values, page_stride, pages, kv_heads, page_tokens, d, table, table_stride, table_width, cu, past, B, room);
+  const ttb_paged_kv kv = KV(keys, values, page_stride, pages, kv_heads, page_tokens, d, table, table_stride, table_width, cu, past, B);
   const ttb_paged_rotary r = {static_cast<const double*>(At(freqs)), rotary_dim, interleaved, scale, At(q), At(q_out), ldq, ldq_out, heads};
-  core::Check(ttb_paged_append(c, dtype, &kv, tokens, At(k), ldk, At(v), ldv, freqs ? &r : nullptr), c, "paged_append");
+  core::Check(ttb_paged_append_room(c, dtype, &kv, tokens, At(k), ldk, At(v), ldv, freqs ? &r : nullptr, Ints(room)), c, "paged_append");
 }
 
 void PagedAttention(int device, Ptr stream, int dtype, Ptr keys, Ptr values, int64_t page_stride, int64_t pages, int64_t kv_heads, int64_t page_tokens, int64_t d,
                     Ptr table, int64_t table_stride, int64_t table_width, Ptr cu, Ptr past, int64_t B, Ptr room, Ptr q, int64_t ldq, int64_t tokens, int64_t heads, bool causal,
                     float scale, Ptr out, int64_t ldo) {
   ttb_ctx* c = OnStream(device, stream);
-  const ttb_paged_kv kv = KV(keys, values, page_stride, pages, kv_heads, page_tokens, d, table, table_stride, table_width, cu, past, B, room);
-  core::Check(ttb_paged_attention(c, dtype, &kv, At(q), ldq, tokens, heads, causal, scale, At(out), ldo), c, "paged_attention");
+  const ttb_paged_kv kv = KV(keys, values, page_stride, pages, kv_heads, page_tokens, d, table, table_stride, table_width, cu, past, B);
+  core::Check(ttb_paged_attention_room(c, dtype, &kv, At(q), ldq, tokens, heads, causal, scale, At(out), ldo, Ints(room)), c, "paged_attention");
 }
 
 void PagedReserve(int device, Ptr stream, Ptr table, int64_t stride, int64_t B, int64_t width, Ptr lens, Ptr refs, int64_t pages, Ptr new_tokens, int64_t page_tokens,
                   Ptr granted, Ptr copies, Ptr room) {
   ttb_ctx* c = OnStream(device, stream);
-  const ttb_paged_tables t = {Ints(table), stride, B, width, Ints(lens), Ints(refs), pages, Ints(room)};
-  core::Check(ttb_paged_reserve(c, &t, Ints(new_tokens), page_tokens, Ints(granted), Ints(copies)), c, "paged_reserve");
+  const ttb_paged_tables t = {Ints(table), stride, B, width, Ints(lens), Ints(refs), pages};
+  core::Check(ttb_paged_reserve_room(c, &t, Ints(new_tokens), page_tokens, Ints(granted), Ints(copies), Ints(room)), c, "paged_reserve");
 }
 
 void PagedFork(int device, Ptr stream, Ptr table, int64_t stride, int64_t B, int64_t width, Ptr lens, Ptr refs, int64_t pages, Ptr parents) {
   ttb_ctx* c = OnStream(device, stream);
-  const ttb_paged_tables t = {Ints(table), stride, B, width, Ints(lens), Ints(refs), pages, nullptr};
+  const ttb_paged_tables t = {Ints(table), stride, B, width, Ints(lens), Ints(refs), pages};
   core::Check(ttb_paged_fork(c, &t, Ints(parents)), c, "paged_fork");
 }
 
@@ -129,7 +129,7 @@ void PagedCopy(int device, Ptr stream, Ptr base, int64_t planes, int64_t plane_s
 void PagedCompact(int device, Ptr stream, Ptr table, int64_t stride, int64_t B, int64_t width, Ptr lens, Ptr refs, int64_t pages, Ptr base, int64_t planes,
                   int64_t plane_stride, int64_t pool_pages, int64_t page_stride, int64_t page_bytes, Ptr used) {
   ttb_ctx* c = OnStream(device, stream);
-  const ttb_paged_tables t = {Ints(table), stride, B, width, Ints(lens), Ints(refs), pages, nullptr};
+  const ttb_paged_tables t = {Ints(table), stride, B, width, Ints(lens), Ints(refs), pages};
   const ttb_paged_pool a = {At(base), planes, plane_stride, pool_pages, page_stride, page_bytes};
   core::Check(ttb_paged_compact(c, &t, &a, Ints(used)), c, "paged_compact");
 }

@@ -371,21 +371,20 @@ struct Tables {
   int B, width, pages;
   int32_t *lens, *refs;
   int* status;
-  int32_t* room;
 };
 
 // Pages for new[b] more tokens of every row (see ttb.h for the rules). One block; thread b decides for row b.
 // A row writes to the columns from the page that it has begun, or else the next one, to the last that its new tokens reach. What it lists there (it may have kept fewer tokens
 // than it once had room for) stays its own; a page in any of them is left for a fresh one only where other rows list it too, unless the row is the last of holders that all
 // write. A row's thread looks at its first columns. What is beyond them (a prompt's) warps fill in; only a row that lists a page in each of its first columns can list more there
-// (nothing is listed behind a row's first -1), and those go by keeper[page], made before the first count changes: looking at all of them took 64 prompts of 4096 tokens from 14 to 23 us.
+// (nothing is listed behind a row's first -1), and those go by keeper[page], made before the first count changes: 64 prompts of 4096 tokens 17 us, and 23 with all columns looked at.
 // 64 rows over 1300 pages, most of them sharing the page that they go on in: 8 us with cold caches.
 // free_list [pages], sharers [pages], keeper [pages]: scratch, not initialised.
 constexpr int kOwnColumns = 2;
 constexpr int kNobody = -1, kUncounted = -2, kWhoever = INT_MAX;  // keeper: all holders leave it; its count is zero, so that it is free; one row alone lists it
 __global__ void __launch_bounds__(kManageThreads, 1)
-paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page_tokens, int32_t* granted, int32_t* copies, int* free_list, int* sharers,
-                     int* keeper) {
+paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page_tokens, int32_t* granted, int32_t* copies, int32_t* room, int* free_list,
+                     int* sharers, int* keeper) {
   __shared__ int scratch[33];
   __shared__ int s_first[kMaxSequences], s_want[kMaxSequences], s_at[kMaxSequences];
   __shared__ bool s_more[kMaxSequences];  // whether a row may list pages beyond its first columns
@@ -504,7 +503,7 @@ paged_reserve_kernel(const Tables t, const int32_t* __restrict__ fresh, int page
   const int c = block_scan(copy ? 1 : 0, scratch, &n_copies);
   if (b < t.B) {
     granted[b] = ok;
-    if (t.room) t.room[b] = ok;
+    if (room) room[b] = ok;
     if (!ok) s_want[b] = first;  // nothing to fill in
     s_at[b] = before + own;
     if (copy) {
@@ -678,7 +677,7 @@ int check_tables(ttb_ctx* ctx, const char* what, const ttb_paged_tables* a, Tabl
   TTB_REQUIRE(ctx, a->B >= 0 && a->B <= kMaxSequences, "%s: at most %d rows", what, kMaxSequences);
   TTB_REQUIRE(ctx, a->width > 0 && a->width < (1ll << 30) && a->stride >= a->width, "%s: bad table width", what);
   TTB_REQUIRE(ctx, a->pages > 0 && a->pages < (1ll << 30), "%s: bad number of pages", what);
-  *t = Tables{a->table, a->stride, (int)a->B, (int)a->width, (int)a->pages, a->lens, a->refs, ctx->d_status, a->room};
+  *t = Tables{a->table, a->stride, (int)a->B, (int)a->width, (int)a->pages, a->lens, a->refs, ctx->d_status};
   return TTB_OK;
 }
 
@@ -732,6 +731,11 @@ extern "C" int ttb_rotary(ttb_ctx* ctx, const ttb_rotary_args* a) {
 
 extern "C" int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv,
                                 const ttb_paged_rotary* r) {
+  return ttb_paged_append_room(ctx, dtype, kv, tokens, k, ldk, v, ldv, r, nullptr);
+}
+
+extern "C" int ttb_paged_append_room(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t tokens, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                     const ttb_paged_rotary* r, const int32_t* room) {
   if (!ctx) return TTB_ERR_INVALID;
   RotaryParams p = {};
   const int bad = check_kv(ctx, "paged_append", dtype, kv, tokens, &p.s);
@@ -759,12 +763,17 @@ extern "C" int ttb_paged_append(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv,
   DeviceGuard g(ctx->device);
   p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
   p.keys = kv->keys; p.values = kv->values; p.page_stride = kv->page_stride;
-  p.room = kv->room;
+  p.room = room;
   p.tokens = (int)tokens;
   return dtype == TTB_F16 ? launch_rotary<__half, true>(ctx, p, "paged_append") : launch_rotary<__nv_bfloat16, true>(ctx, p, "paged_append");
 }
 
 extern "C" int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* a, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies) {
+  return ttb_paged_reserve_room(ctx, a, new_tokens, page_tokens, granted, copies, nullptr);
+}
+
+extern "C" int ttb_paged_reserve_room(ttb_ctx* ctx, const ttb_paged_tables* a, const int32_t* new_tokens, int64_t page_tokens, int32_t* granted, int32_t* copies,
+                                      int32_t* room) {
   if (!ctx) return TTB_ERR_INVALID;
   Tables t;
   const int bad = check_tables(ctx, "paged_reserve", a, &t);
@@ -779,7 +788,8 @@ extern "C" int ttb_paged_reserve(ttb_ctx* ctx, const ttb_paged_tables* a, const 
   int s = ttb_alloc(ctx, (size_t)a->pages * 3 * sizeof(int), "paged_reserve/scratch", &ws);
   if (s) return s;
   int* w = static_cast<int*>(ws);
-  launch_pdl(paged_reserve_kernel, dim3(1), dim3(kManageThreads), 0, ctx->stream, t, new_tokens, (int)page_tokens, granted, copies, w, w + a->pages, w + 2 * a->pages);
+  launch_pdl(paged_reserve_kernel, dim3(1), dim3(kManageThreads), 0, ctx->stream, t, new_tokens, (int)page_tokens, granted, copies, room, w, w + a->pages,
+             w + 2 * a->pages);
   s = launched(ctx, "paged_reserve");
   const int f = ttb_free(ctx, ws, "paged_reserve/scratch");
   return s ? s : f;

@@ -630,6 +630,11 @@ int launch_all(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, int64_t heads, P
 
 extern "C" int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const void* q, int64_t ldq, int64_t tokens, int64_t heads, int causal,
                                    float scale, void* out, int64_t ldo) {
+  return ttb_paged_attention_room(ctx, dtype, kv, q, ldq, tokens, heads, causal, scale, out, ldo, nullptr);
+}
+
+extern "C" int ttb_paged_attention_room(ttb_ctx* ctx, int dtype, const ttb_paged_kv* kv, const void* q, int64_t ldq, int64_t tokens, int64_t heads, int causal,
+                                        float scale, void* out, int64_t ldo, const int32_t* room) {
   if (!ctx) return TTB_ERR_INVALID;
   Params p = {};
   const int bad = check_kv(ctx, "paged_attention", dtype, kv, tokens, &p.s);
@@ -648,7 +653,7 @@ extern "C" int ttb_paged_attention(ttb_ctx* ctx, int dtype, const ttb_paged_kv* 
   p.ldo = ldo;
   p.group = (int)(heads / kv->kv_heads);
   p.scale = scale * kLog2e;
-  p.room = kv->room;
+  p.room = room;
   p.split.causal = causal != 0;
   if (kv->d == 64) return dtype == TTB_F16 ? launch_all<__half, 64>(ctx, dtype, kv, heads, p) : launch_all<__nv_bfloat16, 64>(ctx, dtype, kv, heads, p);
   return dtype == TTB_F16 ? launch_all<__half, 128>(ctx, dtype, kv, heads, p) : launch_all<__nv_bfloat16, 128>(ctx, dtype, kv, heads, p);
