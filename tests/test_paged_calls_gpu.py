@@ -12,7 +12,7 @@ DEV = torch.device("cuda:0")
 
 
 def ints(values):
-    return torch.tensor(values, dtype=torch.int32, device=DEV)
+    return torch.tensor(list(values), dtype=torch.int32, device=DEV)
 
 
 @pytest.fixture
@@ -101,4 +101,43 @@ def test_attention_over_pages_that_rows_share(new, causal):
         want, off = attended(q[t:t + n], pool[0][held, :, at % page], pool[1][held, :, at % page], past[b], causal)
         assert ((got[t:t + n].double() - want).abs() <= off).all()
         t += n
+    assert cxx.device_status(0) == _capi.OK
+
+
+def test_advance_takes_what_can_be_added_to_the_lengths():
+    for counts, want in (([1, 2, 3], [1, 0, 3]), (ints([1, 2, 3]), [1, 0, 3]), (torch.tensor([1, 2, 3], device=DEV), [1, 0, 3]), (4, [4, 0, 4]), (torch.tensor(2), [2, 0, 2]),
+                         (torch.tensor([True, True, False], device=DEV), [1, 0, 0]), (ints([-0]), [0, 0, 0])):
+        cache = tt.PagedKVCache(1, 4, 3, 64, 2, 64, device=DEV)
+        cache.room[1] = 0
+        cache.advance(counts)
+        assert cache.lens.tolist() == want and cache.lens.dtype == torch.int32
+
+
+def test_a_step_captured_without_an_arena():
+    """Workspaces that the graph allocates and frees by itself: replays beside the eager run, a second graph of the same step alive."""
+    B, dtype = 3, torch.float16
+    q, k, v = (torch.randn(B, 2, 64, device=DEV, dtype=dtype) for _ in range(3))
+    cu, ones = ints(range(B + 1)), ints([1] * B)
+
+    def step(c, out):
+        c.reserve(ones)
+        c.append(0, k, v, cu)
+        c.attend(0, q, cu, out=out)
+        c.advance(ones)
+
+    caches, outs, graphs = [tt.PagedKVCache(1, 30, B, 160, 2, 64, 16, dtype, DEV) for _ in range(3)], [torch.zeros_like(q) for _ in range(3)], []
+    step(tt.PagedKVCache(1, 30, B, 160, 2, 64, 16, dtype, DEV), torch.zeros_like(q))  # (a first run loads the kernels)
+    torch.cuda.synchronize()
+    for c, out in list(zip(caches, outs))[1:]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            step(c, out)
+    cxx.set_stream(0, torch.cuda.current_stream().cuda_stream)
+    for _ in range(40):
+        step(caches[0], outs[0])
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for c, out in zip(caches[1:], outs[1:]):
+            assert torch.equal(outs[0], out) and torch.equal(caches[0].lens, c.lens) and torch.equal(caches[0].table, c.table)
     assert cxx.device_status(0) == _capi.OK

@@ -330,7 +330,7 @@ class PagedKVCache:
 
     def advance(self, new_tokens: Union[torch.Tensor, Sequence[int]]) -> None:
         """The new tokens are cached now, those of the sequences that had room. Fewer than were reserved may be kept: the rest of the room stays the sequence's."""
-        self.lens.addcmul_(self._counts(new_tokens), self.room)
+        self.lens.addcmul_(self.room, self._counts(new_tokens))
 
     def fork(self, parents: Union[torch.Tensor, Sequence[int]]) -> None:
         """paged_fork: sequence b becomes what parents[b] was; -1 frees it."""
